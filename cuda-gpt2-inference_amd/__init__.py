@@ -20,8 +20,8 @@ from typing import Optional
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _ROOT = os.path.dirname(_HERE)
 LIB_PATH = os.path.join(_HERE, "libgpt2_mi355x.so")
-SOURCES = ("layernorm.hip", "elementwise.hip", "matmul.hip", "attention.hip", "decode.hip",
-           "gpt2.hip")
+SOURCES = ("layernorm.hip", "elementwise.hip", "matmul.hip", "attention.hip", "paged.hip",
+           "decode.hip", "gpt2.hip")
 HIPCC_FLAGS = (
     "-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-shared",
     # packed-fp32 VALU forms are switched off for every HIP translation unit
@@ -45,6 +45,8 @@ EXPORTS = (
     "matmul_forward_splitk_plan", "matmul_forward_splitk_forced_status",
     "matmul_forward_residual_status", "matmul_forward_first_columns",
     "attention_forward", "attention_forward_status",
+    "kv_store_paged_status", "attention_decode_paged_workspace", "attention_decode_paged_status",
+    "kv_evict_paged_status",
     "argmax_forward", "argmax_forward_status",
     "matmul_forward_argmax_workspace", "matmul_forward_argmax_status",
     "matmul_forward_argmax_noalloc_status",
@@ -96,6 +98,12 @@ class GPT2Config(ctypes.Structure):
     _fields_ = [("max_seq_len", ctypes.c_int), ("vocab_size", ctypes.c_int),
                 ("num_layers", ctypes.c_int), ("num_heads", ctypes.c_int),
                 ("channels", ctypes.c_int)]
+
+
+class GPT2PagedCache(ctypes.Structure):
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("type", ctypes.c_int), ("num_pages", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_size", ctypes.c_int)]
 
 
 # order of the GPT2_PROF_* enum in the header
@@ -153,6 +161,14 @@ def lib() -> ctypes.CDLL:
         L.matmul_forward_residual_status.restype = ci
         L.matmul_forward_splitk_plan.argtypes = [ci] * 4 + [cz] + [ctypes.POINTER(ci)] * 3
         L.matmul_forward_splitk_plan.restype = ci
+        L.kv_store_paged_status.argtypes = [vp, vp, ci, vp, vp, ci, ci, ci]
+        L.kv_store_paged_status.restype = ci
+        L.attention_decode_paged_workspace.argtypes = [vp, ci, ci, ci]
+        L.attention_decode_paged_workspace.restype = cz
+        L.attention_decode_paged_status.argtypes = [vp, vp, vp, ci] + [vp] * 3 + [ci] * 3 + [vp, cz]
+        L.attention_decode_paged_status.restype = ci
+        L.kv_evict_paged_status.argtypes = [vp] * 7 + [ci] * 3
+        L.kv_evict_paged_status.restype = ci
         L.gpt2_create.argtypes, L.gpt2_create.restype = [ctypes.POINTER(GPT2Config)], vp
         L.gpt2_destroy.argtypes, L.gpt2_destroy.restype = [vp], None
         L.gpt2_checkpoint_read_config.argtypes = [ctypes.c_char_p, ctypes.POINTER(GPT2Config)]
@@ -357,6 +373,104 @@ def matmul_forward_splitk_plan(B, T, C, OC, workspace_bytes):
 def attention_forward(out, qkvr, att, inp, B, T, C, NH):
     _check(lib().attention_forward_status(_f32(out), _f32(qkvr), _f32(att), _f32(inp), B, T, C,
                                           NH), "attention_forward")
+
+
+class PagedCache:
+    """A key/value cache in pages (GPT2PagedCache in the header).
+
+    keys, values: contiguous CUDA tensors (num_pages, kv_heads, page_size, head_size) of float32,
+    float16 or bfloat16; table: contiguous int32 CUDA tensor (B, max_pages), the pages of each
+    sequence in order.  The tensors are kept alive and used in place."""
+
+    _TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}  # GPT2HIP_F32, _F16, _BF16
+
+    def __init__(self, keys, values, table):
+        if str(keys.dtype) not in self._TYPES or keys.dtype != values.dtype:
+            raise TypeError(f"keys and values are float32, float16 or bfloat16 alike, got {keys.dtype}, {values.dtype}")
+        if keys.dim() != 4 or keys.shape != values.shape:
+            raise ValueError("keys and values are (num_pages, kv_heads, page_size, head_size) alike, got "
+                             f"{tuple(keys.shape)}, {tuple(values.shape)}")
+        if table.dim() != 2:
+            raise ValueError(f"table is (B, max_pages), got {tuple(table.shape)}")
+        self.keys, self.values, self.table = keys, values, table
+        pages, heads, size, channels = keys.shape
+        self._c = GPT2PagedCache(_ptr(keys), _ptr(values), _i32(table), self._TYPES[str(keys.dtype)], pages,
+                                 size, table.shape[1], heads, channels)
+        self.sequences, self.kv_heads, self.head_size = table.shape[0], heads, channels
+        self.page_size, self.capacity = size, size * table.shape[1]  # capacity: positions per sequence
+        self._ref = ctypes.addressof(self._c)
+
+
+def _has(t, what, *shape):
+    """Refuses a tensor of another shape than the library is going to assume."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what} is {shape}, got {tuple(t.shape)}")
+
+
+def _rows(inp, count, floats):
+    """(pointer, stride in floats) of `count` rows of at least `floats` floats; a view of a wider array will do."""
+    import torch
+    if not isinstance(inp, torch.Tensor) or not inp.is_cuda or inp.dtype != torch.float32:
+        raise TypeError("expected a float32 CUDA tensor of rows")
+    if inp.dim() != 2 or inp.shape[0] < count or inp.shape[1] < floats or (inp.shape[1] > 1 and inp.stride(1) != 1):
+        raise ValueError(f"expected {count} rows of {floats} consecutive floats, got {tuple(inp.shape)} "
+                         f"with strides {inp.stride()}")
+    # the stride of a single row says nothing
+    return inp.data_ptr(), inp.stride(0) if count > 1 else max(inp.stride(0), floats)
+
+
+def kv_store_paged(cache, inp, starts, lengths, N, B, NH):
+    """Store the keys and values of N packed rows (q | k | v; NH = 0: k | v) into the pages: rows
+    starts[b] .. starts[b + 1] - 1 become positions lengths[b] and on of sequence b."""
+    _has(lengths, "lengths", B)
+    _has(starts, "starts", B + 1)
+    if B > cache.sequences:
+        raise ValueError(f"the table lists {cache.sequences} sequences, asked for {B}")
+    rows, stride = _rows(inp, N, (NH + 2 * cache.kv_heads) * cache.head_size)
+    _check(lib().kv_store_paged_status(cache._ref, rows, stride, _i32(starts), _i32(lengths), N, B, NH), "kv_store_paged")
+
+
+def attention_decode_paged_workspace(cache, B, NH, weights=False):
+    """A workspace (uint8 CUDA tensor) that never constrains how attention_decode_paged splits the work."""
+    import torch
+    n = lib().attention_decode_paged_workspace(cache._ref, B, NH, int(weights))
+    if n == 0:
+        raise GPT2HipError(f"attention_decode_paged_workspace: bad arguments B={B} NH={NH} kv_heads={cache.kv_heads}")
+    return torch.empty(n, dtype=torch.uint8, device=cache.keys.device)
+
+
+def attention_decode_paged(out, cache, inp, lengths, B, NH, append=True, weights_in=None, weights_out=None,
+                           workspace=None):
+    """Attention of one new token per sequence over its pages.  append: inp holds packed rows and
+    the new keys and values are stored as position lengths[b] first; otherwise inp holds queries
+    that attend to the lengths[b] positions held.  weights_in, weights_out: accumulated attention
+    weights (B, kv_heads, cache.capacity).  lengths[b] < 0: the row is left as it is."""
+    _has(lengths, "lengths", B)
+    _has(out, "out", B, NH * cache.head_size)
+    if B > cache.sequences:
+        raise ValueError(f"the table lists {cache.sequences} sequences, asked for {B}")
+    for what, w in (("weights_in", weights_in), ("weights_out", weights_out)):
+        if w is not None:
+            _has(w, what, B, cache.kv_heads, cache.capacity)
+    rows, stride = _rows(inp, B, (NH + (2 * cache.kv_heads if append else 0)) * cache.head_size)
+    ws, nbytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
+    _check(lib().attention_decode_paged_status(_f32(out), cache._ref, rows, stride, _i32(lengths), _f32(weights_in),
+                                               _f32(weights_out), B, NH, int(append), ws, nbytes),
+           "attention_decode_paged")
+
+
+def kv_evict_paged(dst, src, kept, weights_out, lengths_out, weights_in, lengths, B, budget, recent):
+    """Bring every sequence down to `budget` positions (the `recent` last ones and the heaviest of the
+    others, each kv head for itself), copied from the pages of src into those of dst."""
+    _has(lengths, "lengths", B)
+    _has(lengths_out, "lengths_out", B)
+    _has(kept, "kept", B, src.kv_heads, budget)
+    _has(weights_in, "weights_in", B, src.kv_heads, src.capacity)
+    _has(weights_out, "weights_out", B, dst.kv_heads, dst.capacity)
+    if B > min(src.sequences, dst.sequences):
+        raise ValueError(f"the tables list {src.sequences} and {dst.sequences} sequences, asked for {B}")
+    _check(lib().kv_evict_paged_status(dst._ref, src._ref, _i32(kept), _f32(weights_out), _i32(lengths_out),
+                                       _f32(weights_in), _i32(lengths), B, budget, recent), "kv_evict_paged")
 
 
 def argmax_forward(ids, logits, N, V):

@@ -213,6 +213,81 @@ int matmul_forward_argmax_status(int* ids, void* workspace, size_t workspace_byt
 int matmul_forward_argmax_noalloc_status(int* ids, const float* inp, const float* weight,
                                          const float* bias, int B, int T, int C, int OC);
 
+/* ---- key/value cache in pages ------------------------------------------------------------
+ * For serving sequences of different lengths (the reference's driver only runs whole batches of
+ * one length, and so does gpt2_prefill / gpt2_decode's dense cache).  keys and values are pools
+ * of num_pages pages, each (kv_heads, page_size, head_size); table is (B, max_pages) int32 on
+ * the device: position p of sequence b is slot p % page_size of page table[b][p / page_size].
+ * Query head h reads kv head h / (NH / kv_heads).  The cache may hold fp32, fp16 or bf16: rows
+ * are rounded to nearest even when they are stored, everything else is computed in fp32.
+ * Any head_size up to 256, any page_size, any kv_heads that divides NH.  A row takes fast paths
+ * where it is a multiple of 16 bytes and keys and values are 16-byte aligned.
+ * lengths (B, int32, on the device) says how many positions each sequence holds; a negative one
+ * marks an unused place in the batch: nothing of it is read or written, and its rows of every
+ * output stay as they were.  Table entries outside [0, num_pages) are never followed: see each
+ * call.  Entries behind a sequence's last position are not read.  Nothing is allocated, nothing
+ * synchronises, nothing is kept between calls: the calls can be captured in a graph. */
+enum { GPT2HIP_F32 = 0, GPT2HIP_F16 = 1, GPT2HIP_BF16 = 2 };
+typedef struct {
+  void* keys;       /* (num_pages, kv_heads, page_size, head_size) of `type`, on the device */
+  void* values;     /* the same shape and type */
+  const int* table; /* (B, max_pages) on the device */
+  int type;         /* GPT2HIP_F32, GPT2HIP_F16 or GPT2HIP_BF16 */
+  int num_pages;
+  int page_size;
+  int max_pages;
+  int kv_heads;
+  int head_size;
+} GPT2PagedCache;
+
+/* Stores the keys and values of N new rows.  inp: packed rows q | k | v of (NH + 2 kv_heads) *
+ * head_size floats (NH = 0: rows hold k | v only), inp_stride floats apart.  Rows starts[b] to
+ * starts[b + 1] - 1 belong to sequence b (starts: B + 1 ascending ints on the device; rows in
+ * front of starts[0] and from starts[B] on belong to nobody and are skipped) and become its
+ * positions lengths[b], lengths[b] + 1, ...; the caller advances lengths.  Positions beyond
+ * max_pages * page_size or on pages that do not exist are not stored.  Two rows for one place
+ * (a page listed twice) leave either. */
+int kv_store_paged_status(const GPT2PagedCache* cache, const float* inp, int inp_stride, const int* starts,
+                          const int* lengths, int N, int B, int NH);
+
+/* Attention of one new token per sequence.  append != 0 (the decode step): inp holds packed rows
+ * q | k | v, inp_stride floats apart, as the qkv product leaves them; the new key and value are
+ * stored as position lengths[b] (the caller advances lengths) and the query attends to positions
+ * 0 .. lengths[b].  append == 0: only the queries of inp are read (rows of NH * head_size floats
+ * or more) and attend to the lengths[b] positions held; with none the row of out is zeros.
+ * out: (B, NH * head_size).  Softmax of q.k / sqrt(head_size), as attention_forward.
+ * weights_in, weights_out (both or neither; may be the same array): (B, kv_heads, max_pages *
+ * page_size) accumulated attention weights, for kv_evict_paged.  weights_out[b][h][i] becomes
+ * weights_in[b][h][i] (0 for the position just appended) plus the weight that position i got
+ * from the query heads of kv head h together; entries behind the last position are not touched.
+ * A sequence that needs a page that does not exist gets NaN (its new row is stored if its own page
+ * exists); so does one whose positions do not fit max_pages * page_size, of which nothing is
+ * stored and whose weights are not touched.
+ * workspace: device memory, 256-byte aligned, for the work to be split over the cache's length;
+ * attention_decode_paged_workspace gives the bytes that never constrain the split (0: bad
+ * arguments).  With less the work is split less, NULL / 0 means not at all, but weights need
+ * what holds B * NH * (max_pages * page_size + head_size + 2) floats.  Its contents do not
+ * matter before and mean nothing after; calls that overlap on one GPU need a workspace each. */
+size_t attention_decode_paged_workspace(const GPT2PagedCache* cache, int B, int NH, int weights);
+int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const float* inp, int inp_stride,
+                                  const int* lengths, const float* weights_in, float* weights_out, int B, int NH,
+                                  int append, void* workspace, size_t workspace_bytes);
+
+/* Brings every (sequence, kv head) down to `budget` positions: the `recent` last ones stay, and
+ * of the others the budget - recent of largest accumulated weight (weights_in, as
+ * attention_decode_paged leaves them; of equal weights the lowest positions stay; a NaN counts
+ * as the largest).  What stays keeps its order and is copied into the pages of dst, which has
+ * the same type, kv_heads and head_size, may be of the same pool, and must list other pages than
+ * src does (a table of src itself is refused).  Sequences of at most `budget` positions are
+ * copied whole.  kept: (B, kv_heads, budget) int32, the position that each place held in src, -1
+ * behind the last; weights_out: (B, kv_heads, dst's max_pages * page_size), the weights of what
+ * stays; lengths_out[b] = min(lengths[b], budget).  budget must fit dst's max_pages * page_size.
+ * A row whose page (in either table) does not exist is not copied and its weight is NaN; a length
+ * beyond src's max_pages * page_size gives -1 in lengths_out and in every entry of kept. */
+int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, int* kept, float* weights_out,
+                          int* lengths_out, const float* weights_in, const int* lengths, int B, int budget,
+                          int recent);
+
 /* ---- whole model: the gpt2_forward driver (llm.c train_gpt2_fp32.cu's
  * gpt2_forward, which the reference plugs its kernels into, README.md:19;
  * dataflow in reference images/gpt2/gpt2_flow.png). ---- */
