@@ -430,13 +430,17 @@ def kv_store_paged(cache, inp, starts, lengths, N, B, NH):
     _check(lib().kv_store_paged_status(cache._ref, rows, stride, _i32(starts), _i32(lengths), N, B, NH), "kv_store_paged")
 
 
+PAGED_COUNTER_BYTES = 65536  # GPT2HIP_PAGED_COUNTER_BYTES
+
+
 def attention_decode_paged_workspace(cache, B, NH, weights=False):
-    """A workspace (uint8 CUDA tensor) that never constrains how attention_decode_paged splits the work."""
+    """A zero-filled workspace (uint8 CUDA tensor) that never constrains how attention_decode_paged
+    splits the work.  Its first PAGED_COUNTER_BYTES stay zero between calls."""
     import torch
     n = lib().attention_decode_paged_workspace(cache._ref, B, NH, int(weights))
     if n == 0:
         raise GPT2HipError(f"attention_decode_paged_workspace: bad arguments B={B} NH={NH} kv_heads={cache.kv_heads}")
-    return torch.empty(n, dtype=torch.uint8, device=cache.keys.device)
+    return torch.zeros(n, dtype=torch.uint8, device=cache.keys.device)
 
 
 def attention_decode_paged(out, cache, inp, lengths, B, NH, append=True, weights_in=None, weights_out=None,

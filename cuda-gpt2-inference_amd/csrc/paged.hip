@@ -9,6 +9,13 @@
 
 #include "common.hpp"
 
+#ifndef G2_MATRIX_FROM
+#define G2_MATRIX_FROM 3
+#endif
+#ifndef G2_RANGE_BYTES
+#define G2_RANGE_BYTES 65536
+#endif
+
 namespace g2 {
 
 typedef _Float16 f16;
@@ -148,20 +155,304 @@ struct AttendPaged {
   const int* lengths;
   const float* weights_in;
   float* weights_out;
-  float *part_o, *part_ml;  // (B, NH, S, HS) and (B, NH, S, 2): unnormalised outputs, (maximum, sum) in the exponent's base-2 scale
-  float* scores;            // (B, NH, capacity) base-2 scores, where weights are asked for
-  int B, NH, G, chunks;     // G query heads per kv head, in `chunks` groups of GQ
-  int stride, S, append;
+  // workspace, where the work is split or weights are asked for
+  unsigned* counters;  // (B, kv_heads, chunks) ranges that have arrived: zero between calls
+  float* part_o;       // (B, NH, S, part_stride) unnormalised outputs of the ranges
+  float* part_ml;      // (B, NH, S, 2) their maxima and sums, in the exponent's base-2 scale
+  float* joined;       // (B, NH, 2) the whole row's
+  float* scores;       // (B, NH, score_stride) base-2 scores
+  int B, NH, G, chunks;  // G query heads per kv head, in `chunks` groups of at most GQ
+  int stride, S, min_range, append;  // at most S ranges, of at least min_range positions
+  int weigh_here;  // weights by the same workgroup (S == 1, chunks == 1)
+  int part_stride, score_stride;
   float scale_log2e;
 };
 
+constexpr int kMaxRanges = 256;
+constexpr int kCounterStride = 32;  // a cache line each: counters that share one are counted one after the other
+
 // How the n positions held by a sequence are dealt to at most S workgroups.
-constexpr int kMinRange = 128;
-__device__ __forceinline__ int range_of(int n, int S) {
-  const int each = (n + S - 1) / S;
-  return each < kMinRange ? kMinRange : (each + 63) & ~63;
+__device__ __forceinline__ int range_of(int n, int S, int min_range) {
+  const int ranges = max(1, min(S, n / min_range));  // none of them small
+  return ((n + ranges - 1) / ranges + 63) & ~63;
 }
 __device__ __forceinline__ int ranges_of(int n, int range) { return n <= range ? 1 : (n + range - 1) / range; }
+
+// exp2(s - above(m)) where m is the running maximum: a maximum of -inf (nothing seen, or only
+// scores of -inf) counts as 0, so that such scores weigh 0 instead of NaN.
+__device__ __forceinline__ float above(float m) { return m == -INFINITY ? 0.f : m; }
+
+// What one workgroup is to do.
+struct Range {
+  int b, kvh, hc, s;         // sequence, kv head, chunk of its query heads, range
+  int head0, heads;          // the chunk's query heads
+  int n, ranges, p0, p1;     // positions held, ranges they are dealt to, this range
+  bool adds;                 // the new row belongs to this range
+};
+
+__device__ __forceinline__ void take_place(const AttendPaged& a, int GQ, Range& w) {
+  int id = blockIdx.x;
+  w.s = id % a.S;
+  id /= a.S;
+  w.hc = id % a.chunks;
+  id /= a.chunks;
+  w.kvh = id % a.pg.kv_heads;
+  w.b = id / a.pg.kv_heads;
+  w.head0 = w.kvh * a.G + w.hc * GQ;
+  w.heads = min(GQ, a.G - w.hc * GQ);
+}
+
+// False where there is nothing (left) to do: unused places, ranges past the last, sequences that
+// do not fit (NaN) or hold nothing (zeros).
+template <int W>
+__device__ __forceinline__ bool take_range(const AttendPaged& a, int tid, Range& w) {
+  w.n = a.lengths[w.b];
+  if (w.n < 0) return false;
+  const bool too_long = w.n > a.pg.capacity - a.append;
+  if (too_long || w.n + a.append == 0) {
+    if (w.s == 0) {
+      const float fill = too_long ? __builtin_nanf("") : 0.f;
+      for (int i = tid; i < w.heads * a.pg.head_size; i += W * kWave)
+        a.out[((size_t)w.b * a.NH + w.head0) * a.pg.head_size + i] = fill;
+    }
+    return false;
+  }
+  const int range = range_of(w.n, a.S, a.min_range);
+  w.ranges = ranges_of(w.n, range);
+  w.p0 = w.s * range;
+  w.p1 = min(w.n, w.p0 + range);
+  w.adds = a.append && w.s == w.ranges - 1;
+  return w.s < w.ranges;
+}
+
+// What the waves of a workgroup hand each other: per wave and head the unnormalised output, the
+// maximum and the sum, and as one more "wave" the new row (sum 1, output its value).  Later the
+// same memory holds what joins the ranges.
+template <int W, int GQ, int ROW>
+struct Meeting {
+  static_assert(ROW % 4 == 0, "rows are read four floats at a time");
+  union {
+    float o[W][GQ][ROW];
+    struct {
+      float weight[GQ][kMaxRanges];
+      f32x4 sum[W * kWave];
+    } join;
+  };
+  float v[ROW];
+  float m[W + 1][GQ], l[W][GQ];
+  float base[GQ], sum[GQ];  // the whole row's, where one workgroup has it all
+  int last;
+};
+
+// 16 bytes of floats at any address that floats may have.
+typedef f32x4 __attribute__((aligned(4))) f32x4_any;
+
+// The new row: rounded as the cache holds it, stored (by the first wave, once per kv head), and
+// scored against the chunk's queries, a head per wave at a time.
+template <class E, int W, int GQ, int ROW>
+__device__ __forceinline__ bool add_row(const AttendPaged& a, const Range& w, int lane, int wave,
+                                        Meeting<W, GQ, ROW>& meet) {
+  constexpr int N = (ROW + 63) / 64;
+  if (wave > 0 && wave >= w.heads) return true;
+  const int HS = a.pg.head_size;
+  const float* row = a.inp + (size_t)w.b * a.stride;
+  const float* kn = row + ((size_t)a.NH + w.kvh) * HS;
+  const float* vn = kn + (size_t)a.pg.kv_heads * HS;
+  bool ok = true;
+  float k[N];
+#pragma unroll
+  for (int j = 0; j < N; j++) k[j] = lane + 64 * j < HS ? kn[lane + 64 * j] : 0.f;
+  if (wave == 0) {
+    const size_t to = (size_t)a.pg.row(w.b, w.kvh, w.n, ok) * HS;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const int d = lane + 64 * j;
+      const E ve = narrow<E>(d < HS ? vn[d] : 0.f);
+      if (d < HS && ok && w.hc == 0) {
+        ((E*)a.pg.keys)[to + d] = narrow<E>(k[j]);
+        ((E*)a.pg.values)[to + d] = ve;
+      }
+      if (d < ROW) meet.v[d] = widen(ve);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; j++) k[j] = widen(narrow<E>(k[j]));
+  for (int g = wave; g < w.heads; g += W) {
+    const float* q = row + (size_t)(w.head0 + g) * HS;
+    float d = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; j++)
+      if (lane + 64 * j < HS) d = fmaf(q[lane + 64 * j] * a.scale_log2e, k[j], d);
+    d = wave_sum(d);
+    if (lane == 0) {
+      meet.m[W][g] = d;
+      if (a.scores) a.scores[((size_t)w.b * a.NH + w.head0 + g) * a.score_stride + w.n] = d;
+    }
+  }
+  return ok;
+}
+
+// Joins the waves and, where the sequence was dealt to several workgroups, the ranges: each leaves
+// its part in the workspace, and whichever of them arrives last (a counter tells it, nobody waits)
+// joins all of them in order, so that the result does not depend on which one that was.  The
+// parts cross XCDs: they are written and read with the cache-bypassing policy, and every wave
+// waits for its stores before the workgroup counts itself in.
+template <int W, int GQ, int ROW>
+__device__ __forceinline__ void finish(const AttendPaged& a, const Range& w, int tid, Meeting<W, GQ, ROW>& meet) {
+  constexpr int THREADS = W * kWave;
+  const int HS = a.pg.head_size, HP4 = a.part_stride >> 2;
+  const size_t bh0 = (size_t)w.b * a.NH + w.head0;
+  const Bypass parts(a.part_o + (w.ranges > 1 ? bh0 * a.S * a.part_stride : 0),
+                     w.ranges > 1 ? (size_t)w.heads * a.S * a.part_stride : 0);
+  __syncthreads();
+  for (int i = tid; i < w.heads * HP4; i += THREADS) {
+    const int g = i / HP4, d = (i - g * HP4) * 4;
+    float top = meet.m[0][g];
+#pragma unroll
+    for (int k = 1; k < W; k++) top = fmaxf(top, meet.m[k][g]);
+    if (w.adds) top = fmaxf(top, meet.m[W][g]);
+    const float base = above(top);
+    float sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+      const float x = __builtin_amdgcn_exp2f(meet.m[k][g] - base);
+      sum = fmaf(x, meet.l[k][g], sum);
+      acc += x * *reinterpret_cast<const f32x4*>(&meet.o[k][g][d]);
+    }
+    if (w.adds) {
+      const float x = __builtin_amdgcn_exp2f(meet.m[W][g] - base);
+      sum += x;
+      acc += x * *reinterpret_cast<const f32x4*>(&meet.v[d]);
+    }
+    if (w.ranges == 1) {
+      float* out = a.out + (bh0 + g) * HS + d;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (d + e < HS) out[e] = acc[e] / sum;
+      if (d == 0 && a.joined) {
+        a.joined[(bh0 + g) * 2] = base;
+        a.joined[(bh0 + g) * 2 + 1] = sum;
+      }
+      if (d == 0) {
+        meet.base[g] = base;
+        meet.sum[g] = sum;
+      }
+    } else {
+      parts.store4((g * a.S + w.s) * a.part_stride + d, acc);
+      if (d == 0) {
+        store_bypass(&a.part_ml[((bh0 + g) * a.S + w.s) * 2], top);
+        store_bypass(&a.part_ml[((bh0 + g) * a.S + w.s) * 2 + 1], sum);
+      }
+    }
+  }
+  if (w.ranges == 1) return;
+  wait_vm();
+  __syncthreads();
+  if (tid == 0) {
+    unsigned* counter = a.counters + kCounterStride * (((size_t)w.b * a.pg.kv_heads + w.kvh) * a.chunks + w.hc);
+    const unsigned old = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool last = old + 1u == (unsigned)w.ranges;
+    if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    meet.last = last;
+  }
+  __syncthreads();
+  if (!meet.last) return;
+  // a wave per head: the ranges' weights, and the sum
+  const int lane = tid & 63;
+  for (int g = tid >> 6; g < w.heads; g += W) {
+    const float* ml = a.part_ml + (bh0 + g) * a.S * 2;
+    float m[kMaxRanges / 64], l[kMaxRanges / 64], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kMaxRanges / 64; k++) {
+      const int s = lane + 64 * k;
+      m[k] = s < w.ranges ? load_bypass(ml + 2 * s) : -INFINITY;
+      l[k] = s < w.ranges ? load_bypass(ml + 2 * s + 1) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxRanges / 64; k++) top = fmaxf(top, m[k]);
+    top = wave_max(top);
+    const float base = above(top);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kMaxRanges / 64; k++) {
+      const float x = __builtin_amdgcn_exp2f(m[k] - base);
+      meet.join.weight[g][lane + 64 * k] = x;
+      sum = fmaf(x, l[k], sum);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) {
+      meet.l[0][g] = sum;
+      if (a.joined) {
+        a.joined[(bh0 + g) * 2] = base;
+        a.joined[(bh0 + g) * 2 + 1] = sum;
+      }
+    }
+  }
+  __syncthreads();
+  // as many threads per four channels as there are to spare, each with every so manieth range
+  int per = 1;
+  while (per < w.heads * HP4 && per < THREADS) per *= 2;
+  const int slices = THREADS / per, slice = tid / per;
+  for (int i0 = 0; i0 < w.heads * HP4; i0 += per) {
+    const int i = i0 + (tid & (per - 1));
+    const bool mine = i < w.heads * HP4;
+    const int g = mine ? i / HP4 : 0, d = mine ? (i - g * HP4) * 4 : 0;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (mine) {
+#pragma unroll 8
+      for (int s = slice; s < w.ranges; s += slices)
+        acc += meet.join.weight[g][s] * parts.load4((g * a.S + s) * a.part_stride + d);
+    }
+    if (slices > 1) {
+      meet.join.sum[tid] = acc;
+      __syncthreads();
+      if (slice == 0)
+        for (int k = 1; k < slices; k++) acc += meet.join.sum[tid + k * per];
+    }
+    if (mine && slice == 0) {
+      const float sum = meet.l[0][g];
+      float* out = a.out + (bh0 + g) * HS + d;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (d + e < HS) out[e] = acc[e] / sum;
+    }
+  }
+}
+
+// weights_out = weights_in + sum over the group's heads of exp2(score - maximum) / sum, where this
+// workgroup has all positions and heads of a kv head.
+template <int W, int GQ, int ROW>
+__device__ __forceinline__ void weigh(const AttendPaged& a, const Range& w, int tid, Meeting<W, GQ, ROW>& meet) {
+  __syncthreads();  // the scores of all waves and meet.base, meet.sum
+  const size_t at = ((size_t)w.b * a.pg.kv_heads + w.kvh) * a.pg.capacity;
+  const float* scores = a.scores + ((size_t)w.b * a.NH + w.head0) * a.score_stride;
+  for (int i = tid; i < w.n + a.append; i += W * kWave) {
+    float x = i < w.n ? a.weights_in[at + i] : 0.f, p = 0.f;
+#pragma unroll 4
+    for (int g = 0; g < w.heads; g++)
+      p += __builtin_amdgcn_exp2f(scores[(size_t)g * a.score_stride + i] - meet.base[g]) / meet.sum[g];
+    a.weights_out[at + i] = x + p;
+  }
+}
+
+// Sums across the four rows of 16 lanes, two values for the price of one: v_permlane32_swap puts
+// x's halves side by side with y's, v_permlane16_swap rows with rows.
+__device__ __forceinline__ float halves_sum(float x, float y) {  // lanes 0-31: x's, lanes 32-63: y's
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+  const unsigned lo = r[0], hi = r[1];
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float rows_sum(float x, float y) {  // rows 0, 2: x's; rows 1, 3: y's
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+  const unsigned lo = r[0], hi = r[1];
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+// The sums of four values over the four rows: row i of 16 lanes receives that of value quad_value(i).
+__device__ __forceinline__ float quads_sum(float x0, float x1, float x2, float x3) {
+  return rows_sum(halves_sum(x0, x1), halves_sum(x2, x3));
+}
+__device__ __forceinline__ int quad_value(int quad) { return quad == 1 ? 2 : quad == 2 ? 1 : quad; }
 
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v) {
@@ -174,113 +465,116 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// exp2(a - m) where m is the running maximum: a maximum of -inf (nothing seen, or only scores of
-// -inf) counts as 0, so that such scores weigh 0 instead of NaN.
-__device__ __forceinline__ float above(float m) { return m == -INFINITY ? 0.f : m; }
-
-constexpr int kAttWaves = 4;
-
-// A workgroup takes one range of positions of one (sequence, kv head) for GQ of the query heads
-// that share it.  LPR lanes hold one row of keys or values, 16 bytes each, so that a wave's load
-// covers 64 / LPR rows; every such group of lanes keeps a softmax (maximum, sum, output) of its
-// own over the rows it has seen, and the groups, the waves and the ranges meet only at the end.
-// SCALAR: rows of any size and alignment, a row per wave, one element per lane and load.
-template <class E, int LPR, int GQ, int U, bool SCALAR>
-__global__ __launch_bounds__(kAttWaves* kWave) void attention_paged_kernel(const AttendPaged a) {
+// One or two query heads per kv head: LPR lanes hold one row of keys or values, 16 bytes each, so
+// that a wave's load covers 64 / LPR rows; every such group of lanes keeps a softmax (maximum,
+// sum, output) of its own over the rows it has seen, and the groups, the waves and the ranges meet
+// only at the end.
+// SCALAR: rows of any size and alignment and any number of heads, GQ at a time: a row per wave,
+// one element per lane and load.
+template <class E, int LPR, int GQ, int U, int W, bool SCALAR>
+__global__ __launch_bounds__(W* kWave) void attention_paged_kernel(const AttendPaged a) {
   constexpr int VEC = SCALAR ? 4 : kPer16<E>;
   constexpr int RPW = 64 / LPR;
   constexpr int TILE = U * RPW;
+  constexpr int ROW = LPR * VEC;
   static_assert(TILE <= 64, "a tile's rows are looked up by one lane each");
+  __shared__ Meeting<W, GQ, ROW> meet;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int sub = lane & (LPR - 1), rg = lane / LPR;
-  const int HS = a.pg.head_size, KVH = a.pg.kv_heads;
-  int id = blockIdx.x;
-  const int s = id % a.S;
-  id /= a.S;
-  const int hc = id % a.chunks;
-  id /= a.chunks;
-  const int kvh = id % KVH, b = id / KVH;
-  const int head0 = kvh * a.G + hc * GQ;
-  const int heads = min(GQ, a.G - hc * GQ);
-
-  const int n = a.lengths[b];
-  if (n < 0) return;  // an unused place in the batch
-  const bool too_long = n > a.pg.capacity - a.append;
-  if (too_long || n + a.append == 0) {
-    if (s == 0) {
-      const float fill = too_long ? __builtin_nanf("") : 0.f;
-      for (int i = tid; i < heads * HS; i += kAttWaves * kWave) a.out[((size_t)b * a.NH + head0) * HS + i] = fill;
-    }
-    return;
-  }
-  const int range = range_of(n, a.S), ranges = ranges_of(n, range);
-  if (s >= ranges) return;
-
+  const int HS = a.pg.head_size;
+  Range w;
+  take_place(a, GQ, w);
   // element j of this lane's part of a row
   auto at = [&](int j) { return SCALAR ? sub + 64 * j : sub * VEC + j; };
+  const bool live = SCALAR || sub * VEC < HS;  // lanes behind the row's end read its last piece and count for nothing
+  const int piece = SCALAR ? 0 : min(sub * VEC, HS - VEC);
   float q[GQ][VEC], o[GQ][VEC], m[GQ], l[GQ];
 #pragma unroll
   for (int g = 0; g < GQ; g++) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int j = 0; j < VEC; j++) {
-      o[g][j] = 0.f;
-      q[g][j] = g < heads && at(j) < HS
-                    ? a.inp[(size_t)b * a.stride + (size_t)(head0 + g) * HS + at(j)] * a.scale_log2e
-                    : 0.f;
-    }
-  }
-
-  auto load = [&](float (&to)[VEC], const void* base, unsigned row) {
-    const E* p = (const E*)base + (size_t)row * HS;
+    const float* src = a.inp + (size_t)w.b * a.stride + (size_t)(w.head0 + (g < w.heads ? g : 0)) * HS;
     if constexpr (SCALAR) {
 #pragma unroll
-      for (int j = 0; j < VEC; j++) to[j] = at(j) < HS ? widen(p[at(j)]) : 0.f;
+      for (int j = 0; j < VEC; j++) q[g][j] = src[min(at(j), HS - 1)];
     } else {
-      u32x4 raw = {0u, 0u, 0u, 0u};
-      if (sub * VEC < HS) raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + sub * VEC));
-      widen16(to, raw, E{});
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) {
+        const f32x4 f = *reinterpret_cast<const f32x4_any*>(src + piece + j);
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[g][j + e] = f[e];
+      }
+    }
+  }
+  if (!take_range<W>(a, tid, w)) return;
+  bool ok = true;
+  const int p1 = w.p1;
+  int t = w.p0 + wave * TILE;
+  // the rows of the tile at `from`, one per lane (behind the range: of its last position)
+  auto look_up = [&](int from) { return a.pg.row(w.b, w.kvh, min(from + (lane & (TILE - 1)), p1 - 1), ok); };
+  unsigned rows = 0, rows_next = 0;
+  if (t < p1) rows = look_up(t);
+  if (t + W * TILE < p1) rows_next = look_up(t + W * TILE);
+
+  // Rows are kept as they are loaded until they are used.  The keys' registers are free once the
+  // scores are known and the values' once they are added up: the next tile's loads go there at
+  // once, so that half of a tile is always under way.
+  typedef typename std::conditional<SCALAR, E[VEC], u32x4>::type Raw;
+  struct Piece {
+    Raw x;
+  };
+  auto load = [&](const void* base, unsigned row) {
+    const E* p = (const E*)base + (size_t)row * HS;
+    Piece r;
+    if constexpr (SCALAR) {
+#pragma unroll
+      for (int j = 0; j < VEC; j++) r.x[j] = p[min(at(j), HS - 1)];
+    } else {
+      r.x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + piece));
+    }
+    return r;
+  };
+  auto unpack = [&](float (&to)[VEC], const Piece& r) {
+    if constexpr (SCALAR) {
+#pragma unroll
+      for (int j = 0; j < VEC; j++) to[j] = at(j) < HS ? widen(r.x[j]) : 0.f;
+    } else {
+      widen16(to, r.x, E{});
     }
   };
-  // The softmax of this lane's row group over U more rows: keys k, values v; sc[g][u] base-2 scores.
-  float* const scores = a.scores ? a.scores + ((size_t)b * a.NH + head0) * a.pg.capacity : nullptr;
+  float* const scores = a.scores ? a.scores + ((size_t)w.b * a.NH + w.head0) * a.score_stride : nullptr;
 
-  const int p0 = s * range, p1 = min(n, p0 + range);
-  bool ok = true;
-  int t = p0 + wave * TILE;
-  unsigned next = t < p1 ? a.pg.row(b, kvh, min(t + (lane & (TILE - 1)), p1 - 1), ok) : 0u;
-  for (; t < p1; t += kAttWaves * TILE) {
-    const unsigned rows = next;
-    if (t + kAttWaves * TILE < p1)
-      next = a.pg.row(b, kvh, min(t + kAttWaves * TILE + (lane & (TILE - 1)), p1 - 1), ok);
-    float k[U][VEC], v[U][VEC];
+  Piece kr[U], vr[U];
+  // one tile; MORE: another follows, so that this one is whole
+  auto step = [&](auto more) {
+    constexpr bool MORE = decltype(more)::value;
+    unsigned rows_after = 0;
+    if constexpr (MORE) {
+      if (t + 2 * W * TILE < p1) rows_after = look_up(t + 2 * W * TILE);
+    }
+    float sc[GQ][U];
 #pragma unroll
-    for (int u = 0; u < U; u++) load(k[u], a.pg.keys, __shfl(rows, u * RPW + rg, 64));
+    for (int u = 0; u < U; u++) {
+      float k[VEC];
+      unpack(k, kr[u]);
+      const bool in = MORE || t + u * RPW + rg < p1;
 #pragma unroll
-    for (int u = 0; u < U; u++) load(v[u], a.pg.values, __shfl(rows, u * RPW + rg, 64));
-    const bool full = t + TILE <= p1;
-    if (!full) {
-      // rows behind the range were read as copies of its last one: they weigh nothing, whatever they hold
+      for (int g = 0; g < GQ; g++) {
+        float d = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; u++)
+        for (int j = 0; j < VEC; j++) d = fmaf(q[g][j], k[j], d);
+        d = row_sum<LPR>(live ? d : 0.f);
+        if (scores && sub == 0 && in && g < w.heads) scores[(size_t)g * a.score_stride + t + u * RPW + rg] = d;
+        sc[g][u] = in ? d : -INFINITY;
+      }
+    }
+    if constexpr (MORE) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) v[u][j] = t + u * RPW + rg < p1 ? v[u][j] : 0.f;
+      for (int u = 0; u < U; u++) kr[u] = load(a.pg.keys, __shfl(rows_next, u * RPW + rg, 64));
     }
 #pragma unroll
     for (int g = 0; g < GQ; g++) {
-      float sc[U], top = m[g];
+      float top = m[g];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        float d = 0.f;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) d = fmaf(q[g][j], k[u][j], d);
-        d = row_sum<LPR>(d);
-        const bool in = t + u * RPW + rg < p1;
-        if (scores && sub == 0 && in && g < heads) scores[(size_t)g * a.pg.capacity + t + u * RPW + rg] = d;
-        sc[u] = in ? d : -INFINITY;
-        top = fmaxf(top, sc[u]);
-      }
+      for (int u = 0; u < U; u++) top = fmaxf(top, sc[g][u]);
       const float base = above(top);
       const float fade = __builtin_amdgcn_exp2f(m[g] - base);
       m[g] = top;
@@ -289,293 +583,685 @@ __global__ __launch_bounds__(kAttWaves* kWave) void attention_paged_kernel(const
       for (int j = 0; j < VEC; j++) o[g][j] *= fade;
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const float p = __builtin_amdgcn_exp2f(sc[u] - base);
-        l[g] += p;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) o[g][j] = fmaf(p, v[u][j], o[g][j]);
+        sc[g][u] = __builtin_amdgcn_exp2f(sc[g][u] - base);
+        l[g] += sc[g][u];
       }
     }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float v[VEC];
+      unpack(v, vr[u]);
+      // rows behind the range were read as copies of its last one: they weigh nothing, whatever they hold
+      if (!MORE && t + u * RPW + rg >= p1) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) v[j] = 0.f;
+      }
+#pragma unroll
+      for (int g = 0; g < GQ; g++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++) o[g][j] = fmaf(sc[g][u], v[j], o[g][j]);
+    }
+    if constexpr (MORE) {
+#pragma unroll
+      for (int u = 0; u < U; u++) vr[u] = load(a.pg.values, __shfl(rows_next, u * RPW + rg, 64));
+      rows_next = rows_after;
+      t += W * TILE;
+    }
+  };
+  if (t < p1) {
+#pragma unroll
+    for (int u = 0; u < U; u++) kr[u] = load(a.pg.keys, __shfl(rows, u * RPW + rg, 64));
+#pragma unroll
+    for (int u = 0; u < U; u++) vr[u] = load(a.pg.values, __shfl(rows, u * RPW + rg, 64));
   }
-
-  // The new row: stored where position n belongs, and attended to as it is stored.
-  if (a.append && s == ranges - 1 && wave == 0) {
-    const float* kn = a.inp + (size_t)b * a.stride + (size_t)a.NH * HS + (size_t)kvh * HS;
-    const float* vn = kn + (size_t)KVH * HS;
-    const unsigned row = a.pg.row(b, kvh, n, ok);
-    float k[VEC], v[VEC];
+  if (w.adds) ok &= add_row<E>(a, w, lane, wave, meet);
+#pragma unroll
+  for (int g = 0; g < GQ; g++) {
+    m[g] = -INFINITY;
+    l[g] = 0.f;
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
-      k[j] = v[j] = 0.f;
-      if (at(j) < HS) {
-        const E ke = narrow<E>(kn[at(j)]), ve = narrow<E>(vn[at(j)]);
-        if (ok && hc == 0 && rg == 0) {
-          ((E*)a.pg.keys)[(size_t)row * HS + at(j)] = ke;
-          ((E*)a.pg.values)[(size_t)row * HS + at(j)] = ve;
-        }
-        k[j] = widen(ke);
-        v[j] = widen(ve);
-      }
+      o[g][j] = 0.f;
+      q[g][j] *= a.scale_log2e;
     }
-#pragma unroll
-    for (int g = 0; g < GQ; g++) {
-      float d = 0.f;
-#pragma unroll
-      for (int j = 0; j < VEC; j++) d = fmaf(q[g][j], k[j], d);
-      d = row_sum<LPR>(d);
-      if (scores && lane == 0 && g < heads) scores[(size_t)g * a.pg.capacity + n] = d;
-      if (rg == 0) {
-        const float top = fmaxf(m[g], d), base = above(top);
-        const float fade = __builtin_amdgcn_exp2f(m[g] - base), p = __builtin_amdgcn_exp2f(d - base);
-        m[g] = top;
-        l[g] = l[g] * fade + p;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) o[g][j] = fmaf(p, v[j], o[g][j] * fade);
-      }
-    }
+  }
+  if (t < p1) {
+    while (t + W * TILE < p1) step(std::true_type{});
+    step(std::false_type{});
   }
 
   // row groups of the wave
-#pragma unroll
-  for (int g = 0; g < GQ; g++)
-#pragma unroll
-    for (int off = LPR; off < 64; off *= 2) {
-      const float mo = __shfl_xor(m[g], off, 64), lo = __shfl_xor(l[g], off, 64);
-      const float top = fmaxf(m[g], mo), base = above(top);
-      const float x = __builtin_amdgcn_exp2f(m[g] - base), y = __builtin_amdgcn_exp2f(mo - base);
-      m[g] = top;
-      l[g] = l[g] * x + lo * y;
-#pragma unroll
-      for (int j = 0; j < VEC; j++) o[g][j] = o[g][j] * x + __shfl_xor(o[g][j], off, 64) * y;
-    }
-  // waves of the workgroup
-  __shared__ float lds_o[kAttWaves][GQ][LPR * VEC], lds_m[kAttWaves][GQ], lds_l[kAttWaves][GQ];
   const bool all_ok = __ballot(!ok) == 0;
-  if (rg == 0) {
 #pragma unroll
-    for (int g = 0; g < GQ; g++) {
+  for (int g = 0; g < GQ; g++) {
+    float top = m[g];
 #pragma unroll
-      for (int j = 0; j < VEC; j++) lds_o[wave][g][at(j)] = o[g][j];
-      if (sub == 0) {
-        lds_m[wave][g] = m[g];
-        lds_l[wave][g] = all_ok ? l[g] : __builtin_nanf("");  // a page that does not exist: NaN, not a stray read
+    for (int off = LPR; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const float fade = __builtin_amdgcn_exp2f(m[g] - above(top));
+    float sum = l[g] * fade;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) o[g][j] *= fade;
+    if constexpr (LPR <= 8) {  // row_ror:8: the two groups of a row of 16 lanes
+      sum += dpp<0x128>(sum);
+#pragma unroll
+      for (int j = 0; j < VEC; j++) o[g][j] += dpp<0x128>(o[g][j]);
+    }
+    if constexpr (LPR <= 16) {
+      sum = quads_sum(sum, sum, sum, sum);
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4) {
+        const float x = quads_sum(o[g][j], o[g][j + 1], o[g][j + 2], o[g][j + 3]);
+        if ((lane & 15) < LPR) meet.o[wave][g][sub * VEC + j + quad_value(lane >> 4)] = x;
       }
+    } else if constexpr (LPR == 32) {
+      sum = halves_sum(sum, sum);
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) meet.o[wave][g][sub * VEC + j + rg] = halves_sum(o[g][j], o[g][j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; j++) meet.o[wave][g][at(j)] = o[g][j];
+    }
+    if (lane == 0) {
+      meet.m[wave][g] = top;
+      meet.l[wave][g] = all_ok ? sum : __builtin_nanf("");  // a page that does not exist: NaN, not a stray read
     }
   }
-  __syncthreads();
-  const size_t bh0 = (size_t)b * a.NH + head0;
-  for (int i = tid; i < heads * HS; i += kAttWaves * kWave) {
-    const int g = i / HS, d = i - g * HS;
-    float top = lds_m[0][g];
-#pragma unroll
-    for (int w = 1; w < kAttWaves; w++) top = fmaxf(top, lds_m[w][g]);
-    const float base = above(top);
-    float sum = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < kAttWaves; w++) {
-      const float x = __builtin_amdgcn_exp2f(lds_m[w][g] - base);
-      sum = fmaf(x, lds_l[w][g], sum);
-      acc = fmaf(x, lds_o[w][g][d], acc);
-    }
-    const size_t bh = bh0 + g;
-    if (ranges == 1)
-      a.out[bh * HS + d] = acc / sum;
-    else
-      a.part_o[(bh * a.S + s) * HS + d] = acc;
-    if (d == 0 && a.part_ml) {
-      a.part_ml[(bh * a.S + s) * 2] = top;
-      a.part_ml[(bh * a.S + s) * 2 + 1] = sum;
-    }
-  }
+  finish(a, w, tid, meet);
+  if (a.weigh_here) weigh(a, w, tid, meet);
 }
 
-constexpr int kJoinPositions = 1024;  // positions per workgroup of the weights' part
+// ---- several query heads per kv head: matrix instructions -----------------------------------
+// Scores and outputs of 16 positions by 16 heads are 16x16 tiles.  Transposed scores
+// S^T = K Q^T: a lane loads 16 bytes of the key row of position (lane % 16), which is an operand
+// as it comes from memory, and receives the scores of four positions 4 (lane / 16) + r for head
+// (lane % 16).  That is at once how the other product wants its left operand: O = P V with V's
+// rows loaded by the lanes of the same four positions.  Neither K, V nor P pass through LDS.
+//
+// The matrix instructions for a 16-bit cache would round the fp32 queries and weights.  So each is
+// cut into as many pieces of 8 (bf16: 3) or 11 (fp16: 2) bits as make up its 24, and their
+// products, exact in fp32, are added up.  Heads beyond the group's are computed on zeros: the
+// kernel is bound by reading the cache (at 16 heads as at 3), not by these instructions.
+template <class E>
+struct Mx;
+template <>
+struct Mx<float> {
+  static constexpr int PIECES = 1;
+};
+template <>
+struct Mx<f16> {
+  static constexpr int PIECES = 2;
+};
+template <>
+struct Mx<bf16> {
+  static constexpr int PIECES = 3;
+};
+constexpr int kMatrixHeads = 16;
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-// Joins the ranges: the first B * NH workgroups the outputs, the others the weights.
-__global__ __launch_bounds__(256) void attention_paged_join_kernel(const AttendPaged a) {
-  const int HS = a.pg.head_size, tid = threadIdx.x;
-  __shared__ float wgt[256], red[256];
-  const bool outputs = (int)blockIdx.x < a.B * a.NH;
-  if (outputs) {
-    const size_t bh = blockIdx.x;
-    const int n = a.lengths[bh / a.NH];
-    if (n < 0 || n > a.pg.capacity - a.append || n + a.append == 0) return;
-    const int ranges = ranges_of(n, range_of(n, a.S));
-    if (ranges == 1) return;  // written already
-    const float* ml = a.part_ml + bh * a.S * 2;
-    red[tid] = tid < ranges ? ml[2 * tid] : -INFINITY;
-    __syncthreads();
-    float top = -INFINITY;
-    for (int s = 0; s < ranges; s++) top = fmaxf(top, red[s]);
-    const float base = above(top);
-    if (tid < ranges) wgt[tid] = __builtin_amdgcn_exp2f(red[tid] - base);
-    __syncthreads();
-    float sum = 0.f;
-    for (int s = 0; s < ranges; s++) sum = fmaf(wgt[s], ml[2 * s + 1], sum);
-    for (int d = tid; d < HS; d += 256) {
-      float acc = 0.f;
-      for (int s = 0; s < ranges; s++) acc = fmaf(wgt[s], a.part_o[(bh * a.S + s) * HS + d], acc);
-      a.out[bh * HS + d] = acc / sum;
-    }
-    return;
+__device__ __forceinline__ unsigned bits_of(float v) { return __builtin_bit_cast(unsigned, v); }
+__device__ __forceinline__ float float_of(unsigned v) { return __builtin_bit_cast(float, v); }
+// the upper, the lower halves of two words as one
+__device__ __forceinline__ unsigned upper_halves(unsigned lo, unsigned hi) {
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+}
+__device__ __forceinline__ unsigned lower_halves(unsigned lo, unsigned hi) {
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+// The pieces of two floats, packed: bf16 by cutting off (8 + 8 + 8 bits are all of a float's 24),
+// fp16 by rounding (11 + 11 bits and two signs leave half a step of fp32 at most).
+__device__ __forceinline__ void cut(unsigned (&to)[3], float a, float b, bf16) {
+  const float a1 = a - float_of(bits_of(a) & 0xffff0000u), b1 = b - float_of(bits_of(b) & 0xffff0000u);
+  const float a2 = a1 - float_of(bits_of(a1) & 0xffff0000u), b2 = b1 - float_of(bits_of(b1) & 0xffff0000u);
+  to[0] = upper_halves(bits_of(a), bits_of(b));
+  to[1] = upper_halves(bits_of(a1), bits_of(b1));
+  to[2] = upper_halves(bits_of(a2), bits_of(b2));
+}
+__device__ __forceinline__ void cut(unsigned (&to)[2], float a, float b, f16) {
+  typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+  const f16x2 hi = {(f16)a, (f16)b};
+  const f16x2 lo = {(f16)(a - (float)hi[0]), (f16)(b - (float)hi[1])};
+  to[0] = __builtin_bit_cast(unsigned, hi);
+  to[1] = __builtin_bit_cast(unsigned, lo);
+}
+
+__device__ __forceinline__ f32x4 mfma32(u32x4 x, u32x4 y, f32x4 c, f16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma32(u32x4 x, u32x4 y, f32x4 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(u32x2 x, u32x2 y, f32x4 c, f16) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, x), __builtin_bit_cast(f16x4, y), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(u32x2 x, u32x2 y, f32x4 c, bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, x), __builtin_bit_cast(s16x4, y), c, 0, 0, 0);
+}
+
+// CPL: output channels per lane (16 CPL cover the head size); P16: 16-position blocks of a tile.
+template <class E, int CPL, int P16, int W>
+__global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const AttendPaged a) {
+  constexpr int GQ = kMatrixHeads, NP = Mx<E>::PIECES;
+  constexpr int PER = kPer16<E>;             // elements per 16 bytes
+  constexpr int ROW = 16 * CPL;              // channels, padded
+  constexpr int KS = ROW / (4 * PER);        // 16-byte loads of a key row's lane
+  constexpr int TILE = 16 * P16;
+  constexpr bool HALF = sizeof(E) == 2;
+  constexpr int VP = CPL < PER ? CPL : PER;  // channels per load of a value row
+  constexpr int VS = CPL / VP;
+  constexpr int VW = VP * (int)sizeof(E) / 4;
+  // fp16 weights are scaled up so that the small ones keep all bits of both pieces
+  constexpr float LIFT = std::is_same<E, f16>::value ? 14.f : 0.f;
+  static_assert(TILE <= 64, "a tile's rows are looked up by one lane each");
+  __shared__ Meeting<W, GQ, ROW> meet;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col = lane & 15, quad = lane >> 4;
+  const int HS = a.pg.head_size;
+  Range w;
+  take_place(a, GQ, w);
+  // queries of head col, channels 4 PER j + PER quad + e
+  f32x4 raw[KS][PER / 4];
+  {
+    const float* src = a.inp + (size_t)w.b * a.stride + (size_t)(w.head0 + (col < w.heads ? col : 0)) * HS;
+#pragma unroll
+    for (int j = 0; j < KS; j++)
+#pragma unroll
+      for (int e = 0; e < PER; e += 4)
+        raw[j][e / 4] = *reinterpret_cast<const f32x4_any*>(src + min(4 * PER * j + PER * quad + e, HS - 4));
   }
-  int id = blockIdx.x - a.B * a.NH;
-  const int per = (a.pg.capacity + kJoinPositions - 1) / kJoinPositions;
-  const int c = id % per;
+  if (!take_range<W>(a, tid, w)) return;
+  bool ok = true;
+  const int p1 = w.p1;
+  int t = w.p0 + wave * TILE;
+  // the rows of the tile at `from`, one per lane (behind the range: of its last position)
+  auto look_up = [&](int from) { return a.pg.row(w.b, w.kvh, min(from + (lane & (TILE - 1)), p1 - 1), ok); };
+  unsigned rows = 0, rows_next = 0;
+  if (t < p1) rows = look_up(t);
+  if (t + W * TILE < p1) rows_next = look_up(t + W * TILE);
+
+  u32x4 q[NP][KS];
+  float unscale = 1.f;
+  auto cut_queries = [&] {
+    float x[KS][PER], most = 0.f;
+#pragma unroll
+    for (int j = 0; j < KS; j++)
+#pragma unroll
+      for (int e = 0; e < PER; e++) {
+        x[j][e] = col < w.heads && 4 * PER * j + PER * quad + e < HS ? raw[j][e / 4][e % 4] * a.scale_log2e : 0.f;
+        most = fmaxf(most, fabsf(x[j][e]));
+      }
+    if constexpr (std::is_same<E, f16>::value) {
+      // a power of two per head takes its largest entry to 2^13 .. 2^14
+      most = fmaxf(most, __shfl_xor(most, 16, 64));
+      most = fmaxf(most, __shfl_xor(most, 32, 64));
+      const int up = 14 - max(-100, min(100, __builtin_amdgcn_frexp_expf(most)));
+      unscale = __builtin_amdgcn_ldexpf(1.f, -up);
+#pragma unroll
+      for (int j = 0; j < KS; j++)
+#pragma unroll
+        for (int e = 0; e < PER; e++) x[j][e] = __builtin_amdgcn_ldexpf(x[j][e], up);
+    }
+#pragma unroll
+    for (int j = 0; j < KS; j++) {
+      if constexpr (HALF) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          unsigned c[NP];
+          cut(c, x[j][2 * e], x[j][2 * e + 1], E{});
+#pragma unroll
+          for (int i = 0; i < NP; i++) q[i][j][e] = c[i];
+        }
+      } else {
+        const f32x4 f = {x[j][0], x[j][1], x[j][2], x[j][3]};
+        q[0][j] = __builtin_bit_cast(u32x4, f);
+      }
+    }
+  };
+
+  f32x4 o[CPL];
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int c = 0; c < CPL; c++) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float* const scores = a.scores && col < w.heads
+                            ? a.scores + ((size_t)w.b * a.NH + w.head0 + col) * a.score_stride : nullptr;
+
+  u32x4 k[P16][KS];
+  unsigned v[P16][4][VS][VW];  // [positions 4 quad + r][piece of the row]
+  auto load_keys = [&](unsigned of) {
+#pragma unroll
+    for (int p = 0; p < P16; p++) {
+      const E* src = (const E*)a.pg.keys + (size_t)__shfl(of, 16 * p + col, 64) * HS;
+#pragma unroll
+      for (int j = 0; j < KS; j++) {
+        // behind the row's end: its last piece, against queries that are 0 there
+        const int d = min(4 * PER * j + PER * quad, HS - PER);
+        k[p][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + d));
+      }
+    }
+  };
+  auto load_values = [&](unsigned of) {
+#pragma unroll
+    for (int p = 0; p < P16; p++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const E* src = (const E*)a.pg.values + (size_t)__shfl(of, 16 * p + 4 * quad + r, 64) * HS;
+#pragma unroll
+        for (int j = 0; j < VS; j++) {
+          // behind the row's end: its last piece, for outputs that nobody takes
+          const int d = min(16 * VP * j + VP * col, HS - VP);
+          if constexpr (VW == 4) {
+            const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + d));
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[p][r][j][e] = x[e];
+          } else {
+            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(src + d));
+            v[p][r][j][0] = x[0];
+            v[p][r][j][1] = x[1];
+          }
+        }
+      }
+  };
+
+  // One tile; MORE: another follows, so that this one is whole.  The keys' registers are free once
+  // the scores are known and the values' once they are added up: the next tile's loads go there at
+  // once, so that half of a tile is always under way.
+  auto step = [&](auto more) {
+    constexpr bool MORE = decltype(more)::value;
+    unsigned rows_after = 0;
+    if constexpr (MORE) {
+      if (t + 2 * W * TILE < p1) rows_after = look_up(t + 2 * W * TILE);
+    }
+    const bool full = MORE || t + TILE <= p1;
+
+    f32x4 sc[P16];
+    if constexpr (HALF) {
+#pragma unroll
+      for (int p = 0; p < P16; p++) sc[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = NP - 1; i >= 0; i--)  // the smallest pieces first
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+#pragma unroll
+          for (int p = 0; p < P16; p++) sc[p] = mfma32(k[p][j], q[i][j], sc[p], E{});
+    } else {
+#pragma unroll
+      for (int p = 0; p < P16; p++) {
+        f32x4 s4[4] = {};  // four chains: a quarter of the roundings in each
+#pragma unroll
+        for (int j = 0; j < KS; j++) {
+          const f32x4 kf = __builtin_bit_cast(f32x4, k[p][j]), qf = __builtin_bit_cast(f32x4, q[0][j]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) s4[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s4[e], 0, 0, 0);
+        }
+        sc[p] = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      }
+    }
+    bool odd = false;
+#pragma unroll
+    for (int p = 0; p < P16; p++) {
+      if constexpr (LIFT != 0.f) sc[p] *= unscale;
+      odd |= __builtin_isunordered(sc[p][0], sc[p][1]) || __builtin_isunordered(sc[p][2], sc[p][3]);
+    }
+    if (__ballot(odd)) {
+      // an infinity in a key has met a 0 (a piece, or behind the row's end): in one piece it would
+      // not have, unless the score is a NaN indeed
+      const float* qs = a.inp + (size_t)w.b * a.stride + (size_t)(w.head0 + (col < w.heads ? col : 0)) * HS;
+#pragma unroll
+      for (int p = 0; p < P16; p++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const E* ks = (const E*)a.pg.keys + (size_t)__shfl(rows, 16 * p + 4 * quad + r, 64) * HS;
+          float x = 0.f;
+          for (int d = 0; d < HS; d++) x = fmaf(qs[d] * a.scale_log2e, widen(ks[d]), x);
+          sc[p][r] = x;
+        }
+    }
+    if constexpr (MORE) load_keys(rows_next);
+    if (scores) {
+#pragma unroll
+      for (int p = 0; p < P16; p++) {
+        float* to = scores + t + 16 * p + 4 * quad;
+        if (full)
+          *reinterpret_cast<f32x4*>(to) = sc[p];
+        else
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+            if (t + 16 * p + 4 * quad + r < p1) to[r] = sc[p][r];
+      }
+    }
+    if (!full) {
+      // rows behind the range are copies of its last one: they weigh nothing, whatever they hold
+#pragma unroll
+      for (int p = 0; p < P16; p++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (t + 16 * p + 4 * quad + r >= p1) {
+            sc[p][r] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < VS; j++)
+#pragma unroll
+              for (int e = 0; e < VW; e++) v[p][r][j][e] = 0u;
+          }
+    }
+
+    // the maximum over all positions of the tile: a head's outputs are added up over them
+    float top = m;
+#pragma unroll
+    for (int p = 0; p < P16; p++) top = fmaxf(top, fmaxf(fmaxf(sc[p][0], sc[p][1]), fmaxf(sc[p][2], sc[p][3])));
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if (__ballot(top > m)) {
+      const float fade = __builtin_amdgcn_exp2f(m - above(top));
+      l *= fade;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float f = __shfl(fade, 4 * quad + r, 64);
+#pragma unroll
+        for (int c = 0; c < CPL; c++) o[c][r] *= f;
+      }
+      m = top;
+    }
+    const float base = above(m) - LIFT;
+#pragma unroll
+    for (int p = 0; p < P16; p++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        sc[p][r] = __builtin_amdgcn_exp2f(sc[p][r] - base);
+        l += sc[p][r];
+      }
+
+    if constexpr (!HALF) {
+#pragma unroll
+      for (int p = 0; p < P16; p++)
+#pragma unroll
+        for (int j = 0; j < VS; j++)
+#pragma unroll
+          for (int e = 0; e < VP; e++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              o[j * VP + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(sc[p][r], float_of(v[p][r][j][e]), o[j * VP + e], 0, 0, 0);
+    } else {
+      // two blocks of positions make one product of 32, where there are two
+      constexpr int PP = P16 % 2 == 0 ? 2 : 1;
+#pragma unroll
+      for (int p = 0; p < P16; p += PP) {
+        unsigned wt[NP][2 * PP];
+#pragma unroll
+        for (int h = 0; h < PP; h++) {
+          unsigned c01[NP], c23[NP];
+          cut(c01, sc[p + h][0], sc[p + h][1], E{});
+          cut(c23, sc[p + h][2], sc[p + h][3], E{});
+#pragma unroll
+          for (int i = 0; i < NP; i++) {
+            wt[i][2 * h] = c01[i];
+            wt[i][2 * h + 1] = c23[i];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VS; j++)
+#pragma unroll
+          for (int e = 0; e < VW; e++) {
+            unsigned even[2 * PP], odds[2 * PP];
+#pragma unroll
+            for (int h = 0; h < PP; h++) {
+              const auto& x = v[p + h];
+              even[2 * h] = lower_halves(x[0][j][e], x[1][j][e]);
+              even[2 * h + 1] = lower_halves(x[2][j][e], x[3][j][e]);
+              odds[2 * h] = upper_halves(x[0][j][e], x[1][j][e]);
+              odds[2 * h + 1] = upper_halves(x[2][j][e], x[3][j][e]);
+            }
+            f32x4 &oe = o[j * VP + 2 * e], &oo = o[j * VP + 2 * e + 1];
+#pragma unroll
+            for (int i = NP - 1; i >= 0; i--) {
+              if constexpr (PP == 2) {
+                const u32x4 l4 = {wt[i][0], wt[i][1], wt[i][2], wt[i][3]};
+                oe = mfma32(l4, u32x4{even[0], even[1], even[2], even[3]}, oe, E{});
+                oo = mfma32(l4, u32x4{odds[0], odds[1], odds[2], odds[3]}, oo, E{});
+              } else {
+                const u32x2 l2 = {wt[i][0], wt[i][1]};
+                oe = mfma16(l2, u32x2{even[0], even[1]}, oe, E{});
+                oo = mfma16(l2, u32x2{odds[0], odds[1]}, oo, E{});
+              }
+            }
+          }
+      }
+    }
+    if constexpr (MORE) {
+      load_values(rows_next);
+      rows = rows_next;
+      rows_next = rows_after;
+      t += W * TILE;
+    }
+  };
+  if (t < p1) {
+    load_keys(rows);
+    load_values(rows);
+  }
+  if (w.adds) ok &= add_row<E>(a, w, lane, wave, meet);
+  cut_queries();
+  if (t < p1) {
+    while (t + W * TILE < p1) step(std::true_type{});
+    step(std::false_type{});
+  }
+
+  // row 4 quad + r of o is head 4 quad + r
+  const bool all_ok = __ballot(!ok) == 0;
+  l = quads_sum(l, l, l, l);
+  if (quad == 0) {
+    meet.m[wave][col] = m == -INFINITY ? m : m - LIFT;
+    meet.l[wave][col] = all_ok ? l : __builtin_nanf("");  // a page that does not exist: NaN, not a stray read
+  }
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+    if (4 * quad + r < w.heads) {
+#pragma unroll
+      for (int j = 0; j < VS; j++)
+#pragma unroll
+        for (int e = 0; e < VP; e++) meet.o[wave][4 * quad + r][16 * VP * j + VP * col + e] = o[j * VP + e][r];
+    }
+  finish(a, w, tid, meet);
+  if (a.weigh_here) weigh(a, w, tid, meet);
+}
+
+constexpr int kWeighPositions = 256;  // positions per workgroup
+
+// The same where the work is split: a thread per position.
+__global__ __launch_bounds__(kWeighPositions) void attention_paged_weights_kernel(const AttendPaged a) {
+  const int per = (a.pg.capacity + kWeighPositions - 1) / kWeighPositions;
+  int id = blockIdx.x;
+  const int i = (id % per) * kWeighPositions + threadIdx.x;
   id /= per;
   const int kvh = id % a.pg.kv_heads, b = id / a.pg.kv_heads;
   const int n = a.lengths[b];
-  if (n < 0 || n > a.pg.capacity - a.append || n + a.append <= c * kJoinPositions) return;
-  const int total = n + a.append, ranges = ranges_of(n, range_of(n, a.S));
-  float w[kJoinPositions / 256] = {};
-  for (int g = 0; g < a.G; g++) {
-    const size_t bh = (size_t)b * a.NH + kvh * a.G + g;
-    const float* ml = a.part_ml + bh * a.S * 2;
-    float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < ranges; s++) top = fmaxf(top, ml[2 * s]);
-    const float base = above(top);
-    for (int s = 0; s < ranges; s++) sum = fmaf(__builtin_amdgcn_exp2f(ml[2 * s] - base), ml[2 * s + 1], sum);
-#pragma unroll
-    for (int j = 0; j < kJoinPositions / 256; j++) {
-      const int i = c * kJoinPositions + j * 256 + tid;
-      if (i < total) w[j] += __builtin_amdgcn_exp2f(a.scores[bh * a.pg.capacity + i] - base) / sum;
-    }
-  }
-  const size_t at = ((size_t)b * a.pg.kv_heads + kvh) * a.pg.capacity;
-#pragma unroll
-  for (int j = 0; j < kJoinPositions / 256; j++) {
-    const int i = c * kJoinPositions + j * 256 + tid;
-    if (i < total) a.weights_out[at + i] = i < n ? a.weights_in[at + i] + w[j] : w[j];
-  }
+  if (n < 0 || n > a.pg.capacity - a.append || i >= n + a.append) return;
+  const size_t at = ((size_t)b * a.pg.kv_heads + kvh) * a.pg.capacity + i;
+  const size_t bh = (size_t)b * a.NH + kvh * a.G;
+  const float x = i < n ? a.weights_in[at] : 0.f;
+  float p = 0.f;
+#pragma unroll 8
+  for (int g = 0; g < a.G; g++)
+    p += __builtin_amdgcn_exp2f(a.scores[(bh + g) * a.score_stride + i] - a.joined[(bh + g) * 2]) / a.joined[(bh + g) * 2 + 1];
+  a.weights_out[at] = x + p;
 }
 
 // ---- kv_evict_paged -------------------------------------------------------------------------
-// The order of weights as unsigned integers: -0 equals 0, and a NaN is the largest of all.
+// The order of weights as unsigned integers: -0 equals 0, and a NaN is the largest of all.  No
+// weight has rank 0.
 __device__ __forceinline__ unsigned rank_of(float w) {
   const unsigned u = __builtin_bit_cast(unsigned, w + 0.0f);
   return w != w ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kPickWaves = 16;
+__device__ __forceinline__ int wave_sum_int(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+constexpr int kFew = 4096;  // ranks that are worth a list of their own
 
 // One workgroup per (sequence, kv head) chooses the positions that stay: the `recent` last ones
 // and, of the others, the budget - recent of largest weight.  The smallest rank that stays is
-// found two bits at a time by counting how many ranks reach each of three candidates (ballots:
-// no histogram, no atomics on data, the same result on every run); a wave owns consecutive
-// positions, so that the places in the output follow from counts alone.  R ranks per thread are
-// kept in registers; R = 0: any length, read again for every count.
-template <int R>
-__global__ __launch_bounds__(kPickWaves* kWave) void kv_evict_pick_kernel(
+// found two bits at a time by counting how many ranks reach each of three candidates: sums of
+// integers, the same on every run.  Once few ranks are left that could be it, they are listed in
+// LDS and the rest is not looked at again until the end; the search ends early where a candidate
+// is reached by exactly as many as are wanted.  A wave owns consecutive positions, so that the
+// places in the output follow from counts alone.  R ranks per thread are kept in registers;
+// R = 0: any length, read again for every count.
+template <int WAVES, int R>
+__global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
     int* __restrict__ kept, int* __restrict__ lengths_out, const float* __restrict__ weights,
     const int* __restrict__ lengths, int KVH, int capacity, int budget, int recent) {
+  constexpr int THREADS = WAVES * kWave;
+  constexpr bool LISTS = R == 0 || R * THREADS > 2 * kFew;
+  constexpr int FEW = LISTS ? kFew / THREADS : 1;
+  __shared__ unsigned list[LISTS ? kFew : 1];
+  __shared__ int counts[16][3], waves[2][WAVES], listed;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t bh = blockIdx.x;
   const int b = (int)(bh / KVH);
+  if (tid < 48) (&counts[0][0])[tid] = 0;
+  if (tid == 0) listed = 0;
   const int n = lengths[b];
   if (n < 0) return;
   const bool too_long = n > capacity;
   const int stay = too_long ? 0 : min(n, budget);
   if (bh % KVH == 0 && tid == 0) lengths_out[b] = too_long ? -1 : stay;
   int* out = kept + bh * budget;
-  for (int j = stay + tid; j < budget; j += kPickWaves * kWave) out[j] = -1;
+  for (int j = stay + tid; j < budget; j += THREADS) out[j] = -1;
   if (stay == n || too_long) {  // nothing has to go
-    for (int j = tid; j < stay; j += kPickWaves * kWave) out[j] = j;
+    for (int j = tid; j < stay; j += THREADS) out[j] = j;
     return;
   }
   const int older = n - recent, want = budget - recent;  // want < older
-  for (int j = tid; j < recent; j += kPickWaves * kWave) out[want + j] = older + j;
+  for (int j = tid; j < recent; j += THREADS) out[want + j] = older + j;
   if (want == 0) return;
 
   const float* w = weights + bh * capacity;
-  const int span = R ? 64 * R : ((older + kPickWaves - 1) / kPickWaves + 63) & ~63;
-  const int first = wave * span, groups = span / 64;
+  const int span = R ? 64 * R : ((older + WAVES - 1) / WAVES + 63) & ~63;
+  const int first = wave * span, groups = R ? R : span / 64;
   unsigned rank[R ? R : 1];
   if constexpr (R > 0) {
+    float x[R];
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-      const int i = first + r * 64 + lane;
-      rank[r] = i < older ? rank_of(w[i]) : 0u;
-    }
+    for (int r = 0; r < R; r++) x[r] = w[min(first + r * 64 + lane, older - 1)];
+#pragma unroll
+    for (int r = 0; r < R; r++) rank[r] = first + r * 64 + lane < older ? rank_of(x[r]) : 0u;
   }
-  // group r of this wave's ranks; 0, which no weight has, behind the last position
-  auto get = [&](int r) -> unsigned {
-    const int i = first + r * 64 + lane;
-    return i < older ? rank_of(w[i]) : 0u;
-  };
-  __shared__ int counts[16][3], waves[2][kPickWaves];
-  if (tid < 48) (&counts[0][0])[tid] = 0;
-  __syncthreads();
-  unsigned low = 0u;
-  for (int step = 0; step < 16; step++) {
-    const int shift = 30 - 2 * step;
-    int c1 = 0, c2 = 0, c3 = 0;
-    const unsigned t1 = low | (1u << shift), t2 = low | (2u << shift), t3 = low | (3u << shift);
+  // calls f(group, its ranks): 0, which no weight has, behind the last position
+  auto each = [&](auto f) {
     if constexpr (R > 0) {
 #pragma unroll
-      for (int r = 0; r < R; r++) {
-        c1 += __popcll(__ballot(rank[r] >= t1));
-        c2 += __popcll(__ballot(rank[r] >= t2));
-        c3 += __popcll(__ballot(rank[r] >= t3));
-      }
+      for (int r = 0; r < R; r++) f(r, rank[r]);
     } else {
+#pragma unroll 8
       for (int r = 0; r < groups; r++) {
-        const unsigned x = get(r);
-        c1 += __popcll(__ballot(x >= t1));
-        c2 += __popcll(__ballot(x >= t2));
-        c3 += __popcll(__ballot(x >= t3));
+        const int i = first + r * 64 + lane;
+        f(r, i < older ? rank_of(w[i]) : 0u);
       }
     }
-    if (lane == 0) {
-      atomicAdd(&counts[step][0], c1);
-      atomicAdd(&counts[step][1], c2);
-      atomicAdd(&counts[step][2], c3);
-    }
-    __syncthreads();
-    low = counts[step][2] >= want ? t3 : counts[step][1] >= want ? t2 : counts[step][0] >= want ? t1 : low;
-  }
-  // low is the smallest rank that stays: all above it, and of its equals as many as there is room for
-  int gt = 0, eq = 0;
-  if constexpr (R > 0) {
+  };
+  unsigned few[FEW];
+  bool from_list = false;
+  __syncthreads();
+
+  unsigned low = 0u;              // at least `want` ranks reach it ...
+  int reach = older, over = 0;    // ... this many; and this many are too large to be the one sought
+  int unlisted = 0;               // how many of those are not on the list
+  for (int step = 0; step < 16 && reach != want; step++) {
+    const int shift = 30 - 2 * step;
+    const unsigned t1 = low | (1u << shift), t2 = low | (2u << shift), t3 = low | (3u << shift);
+    int c1 = 0, c2 = 0, c3 = 0;
+    auto count = [&](unsigned x) {
+      c1 += x >= t1;
+      c2 += x >= t2;
+      c3 += x >= t3;
+    };
+    if (LISTS && from_list) {
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-      gt += __popcll(__ballot(rank[r] > low));
-      eq += __popcll(__ballot(rank[r] == low));
+      for (int k = 0; k < FEW; k++) count(few[k]);
+    } else {
+      each([&](int, unsigned x) { count(x); });
     }
-  } else {
-    for (int r = 0; r < groups; r++) {
-      const unsigned x = get(r);
-      gt += __popcll(__ballot(x > low));
-      eq += __popcll(__ballot(x == low));
+    c1 = wave_sum_int(c1);
+    c2 = wave_sum_int(c2);
+    c3 = wave_sum_int(c3);
+    if (lane < 3) atomicAdd(&counts[step][lane], lane == 0 ? c1 : lane == 1 ? c2 : c3);
+    __syncthreads();
+    c1 = counts[step][0] + unlisted;
+    c2 = counts[step][1] + unlisted;
+    c3 = counts[step][2] + unlisted;
+    if (c3 >= want) {
+      low = t3;
+      reach = c3;
+    } else if (c2 >= want) {
+      low = t2;
+      reach = c2;
+      over = c3;
+    } else if (c1 >= want) {
+      low = t1;
+      reach = c1;
+      over = c2;
+    } else {
+      over = c1;
+    }
+    if constexpr (LISTS) {
+      if (!from_list && reach - over <= kFew && reach != want) {
+        each([&](int, unsigned x) {
+          const bool in = x >= low && x - low < (1u << shift);
+          const unsigned long long m = __ballot(in);
+          if (m) {
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&listed, __popcll(m));
+            at = __shfl(at, 0, 64) + __popcll(m & ((1ull << lane) - 1ull));
+            if (in) list[at] = x;
+          }
+        });
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < FEW; k++) few[k] = k * THREADS + tid < listed ? list[k * THREADS + tid] : 0u;
+        from_list = true;
+        unlisted = over;
+      }
     }
   }
+
+  // all ranks above low stay, and of its equals as many as there is room for
+  int gt = 0, eq = 0;
+  each([&](int, unsigned x) {
+    gt += x > low;
+    eq += x == low;
+  });
+  gt = wave_sum_int(gt);
+  eq = wave_sum_int(eq);
   if (lane == 0) {
     waves[0][wave] = gt;
     waves[1][wave] = eq;
   }
   __syncthreads();
   int above_all = 0, gt_before = 0, eq_before = 0;
-  for (int i = 0; i < kPickWaves; i++) {
+#pragma unroll
+  for (int i = 0; i < WAVES; i++) {
     above_all += waves[0][i];
-    if (i < wave) {
-      gt_before += waves[0][i];
-      eq_before += waves[1][i];
-    }
+    gt_before += i < wave ? waves[0][i] : 0;
+    eq_before += i < wave ? waves[1][i] : 0;
   }
-  const int room = want - above_all;  // for ranks that equal low: the lowest positions have it
+  const int room = want - above_all;  // the lowest positions have it
   const unsigned long long before = (1ull << lane) - 1ull;
-  auto place = [&](int r, unsigned x) {
+  each([&](int r, unsigned x) {
     const unsigned long long g = __ballot(x > low), e = __ballot(x == low);
     const int eq_at = eq_before + __popcll(e & before);
-    const bool stays = x > low || (x == low && eq_at < room);
-    if (stays) out[gt_before + __popcll(g & before) + min(eq_at, room)] = first + r * 64 + lane;
+    const int at = gt_before + __popcll(g & before) + min(eq_at, room);
+    if ((x > low || (x == low && eq_at < room)) && at < want) out[at] = first + r * 64 + lane;
     gt_before += __popcll(g);
     eq_before += __popcll(e);
-  };
-  if constexpr (R > 0) {
-#pragma unroll
-    for (int r = 0; r < R; r++) place(r, rank[r]);
-  } else {
-    for (int r = 0; r < groups; r++) place(r, get(r));
-  }
+  });
 }
 
 // Copies what stays into the pages of the other table: a wave moves the keys and values of ROWS
@@ -601,9 +1287,9 @@ __global__ __launch_bounds__(256) void kv_evict_copy_kernel(Pages dst, Pages src
   bool ok = j < stay;
   if (ok) {
     const int i = kept[bh * budget + j];
-    from = src.row(b, h, i, ok);
+    from = src.row(b, h, min(max(i, 0), n - 1), ok);
     to = dst.row(b, h, j, ok);
-    weights_out[bh * dst.capacity + j] = ok ? weights_in[bh * src.capacity + i] : __builtin_nanf("");
+    weights_out[bh * dst.capacity + j] = ok ? weights_in[bh * src.capacity + min(max(i, 0), n - 1)] : __builtin_nanf("");
   }
   const unsigned long long live = __ballot(ok);
   const int units = row_bytes / UNIT, per = 64 / units > 0 ? 64 / units : 1;  // rows per load
@@ -614,9 +1300,10 @@ __global__ __launch_bounds__(256) void kv_evict_copy_kernel(Pages dst, Pages src
     for (int c = lane % units; c < units; c += 64) {
       const size_t x = (size_t)f * row_bytes + (size_t)c * UNIT, y = (size_t)t * row_bytes + (size_t)c * UNIT;
       if constexpr (UNIT == 16) {
-        const u32x4 kk = *(const u32x4*)((const char*)src.keys + x), vv = *(const u32x4*)((const char*)src.values + x);
-        *(u32x4*)((char*)dst.keys + y) = kk;
-        *(u32x4*)((char*)dst.values + y) = vv;
+        const u32x4 kk = __builtin_nontemporal_load((const u32x4*)((const char*)src.keys + x));
+        const u32x4 vv = __builtin_nontemporal_load((const u32x4*)((const char*)src.values + x));
+        __builtin_nontemporal_store(kk, (u32x4*)((char*)dst.keys + y));
+        __builtin_nontemporal_store(vv, (u32x4*)((char*)dst.values + y));
       } else {
         typedef typename std::conditional<UNIT == 4, unsigned, unsigned short>::type W;
         const W kk = *(const W*)((const char*)src.keys + x), vv = *(const W*)((const char*)src.values + x);
@@ -673,50 +1360,93 @@ static void launch_store(const Pages& pg, const float* inp, int stride, const in
     hipLaunchKernelGGL((kv_store_paged_kernel<E, 1>), grid, block, 0, stream(), pg, inp, stride, starts, lengths, N, B, NH);
 }
 
-// Query heads that one workgroup takes at once.
-static int heads_at_once(int G) { return G >= 5 ? 8 : G >= 3 ? 4 : G; }
+// Which kernel a problem takes, and how it is cut up.
+struct AttendPlan {
+  bool rows16, matrix;
+  int gq, chunks, S, min_range, waves;
+};
 
-// Ranges that a sequence's positions may be split into: enough workgroups to fill the chip.
-constexpr int kMaxRanges = 256;
-static int ranges_for(int B, int KVH, int G, int capacity) {
-  const int gq = heads_at_once(G);
-  const long long groups = (long long)B * KVH * ((G + gq - 1) / gq);
-  const long long want = (2048 + groups - 1) / groups;
-  const long long most = (capacity + kMinRange - 1) / kMinRange;
-  const long long s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > kMaxRanges ? kMaxRanges : s);
+static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
+  AttendPlan p;
+  const int G = NH / c->kv_heads;
+  p.rows16 = rows_by_16(c);
+  p.matrix = p.rows16 && G >= G2_MATRIX_FROM;
+  p.gq = p.matrix ? kMatrixHeads : G >= 3 ? 4 : G;
+  p.chunks = (G + p.gq - 1) / p.gq;
+  const long long groups = (long long)B * c->kv_heads * p.chunks;
+  // few groups: large workgroups, whose waves need no memory to meet
+  const bool wide = groups <= 512;
+  p.waves = wide && p.rows16 && !(p.matrix && c->head_size > 128) ? 8 : 4;
+  // One workgroup per compute unit, or two where each has enough to do: the longest sequence's
+  // workgroups must not outlast the others'.  A range is worth a workgroup from 64 KB on.
+  const long long row_bytes = 2LL * c->head_size * type_bytes(c->type), capacity = (long long)c->max_pages * c->page_size;
+  p.min_range = (int)((G2_RANGE_BYTES / row_bytes + 63) & ~63LL);
+  if (p.min_range < 128) p.min_range = 128;
+  long long S = 512 / groups;
+  if (S < 1 || capacity * row_bytes / S < 512 * 1024) S = 256 / groups;
+  const long long most = (capacity + p.min_range - 1) / p.min_range;
+  if (S > most) S = most;
+  if (groups * kCounterStride * 4 > GPT2HIP_PAGED_COUNTER_BYTES) S = 1;
+  p.S = (int)(S < 1 ? 1 : S > kMaxRanges ? kMaxRanges : S);
+  return p;
 }
 
-static size_t part_bytes(int B, int NH, int HS, int S) { return (size_t)B * NH * S * (HS + 2) * sizeof(float); }
-static size_t score_bytes(int B, int NH, int capacity) { return (size_t)B * NH * capacity * sizeof(float); }
-
-template <class E, int LPR, bool SCALAR>
-static void launch_attend(const AttendPaged& a, unsigned blocks) {
-  const dim3 grid(blocks), block(kAttWaves * kWave);
-  const int gq = heads_at_once(a.G);
-  if (gq == 1)
-    hipLaunchKernelGGL((attention_paged_kernel<E, LPR, 1, 8, SCALAR>), grid, block, 0, stream(), a);
-  else if (gq == 2)
-    hipLaunchKernelGGL((attention_paged_kernel<E, LPR, 2, 8, SCALAR>), grid, block, 0, stream(), a);
-  else if (gq == 4)
-    hipLaunchKernelGGL((attention_paged_kernel<E, LPR, 4, 4, SCALAR>), grid, block, 0, stream(), a);
-  else
-    hipLaunchKernelGGL((attention_paged_kernel<E, LPR, 8, 4, SCALAR>), grid, block, 0, stream(), a);
-}
+// What a call puts into the workspace behind the counters.
+struct AttendSpace {
+  size_t part, ml, joined, scores, total;  // offsets in floats
+  AttendSpace(int B, int NH, int part_stride, int score_stride, int S, bool weights) {
+    const size_t rows = (size_t)B * NH;
+    part = 0;
+    ml = part + (S > 1 ? rows * S * part_stride : 0);
+    joined = ml + (S > 1 ? rows * S * 2 : 0);
+    scores = (joined + (weights ? rows * 2 : 0) + 3) & ~(size_t)3;
+    total = scores + (weights ? rows * score_stride : 0);
+  }
+};
 
 template <class E>
-static void launch_attend(const AttendPaged& a, unsigned blocks, bool vec) {
-  const int lanes = (a.pg.head_size + kPer16<E> - 1) / kPer16<E>;
-  if (!vec)
-    launch_attend<E, 64, true>(a, blocks);
-  else if (lanes <= 8)
-    launch_attend<E, 8, false>(a, blocks);
-  else if (lanes <= 16)
-    launch_attend<E, 16, false>(a, blocks);
-  else if (lanes <= 32)
-    launch_attend<E, 32, false>(a, blocks);
-  else if constexpr (sizeof(E) == 4)
-    launch_attend<E, 64, false>(a, blocks);
+static void launch_attend(const AttendPaged& a, const AttendPlan& p, unsigned blocks) {
+  const int HS = a.pg.head_size, lanes = (HS + kPer16<E> - 1) / kPer16<E>;
+#define G2_KERNEL(W, ...) hipLaunchKernelGGL((__VA_ARGS__), dim3(blocks), dim3(W * kWave), 0, stream(), a)
+#define G2_MATRIX(CPL, P16)                                            \
+  if (p.waves == 8)                                                    \
+    G2_KERNEL(8, attention_paged_matrix_kernel<E, CPL, P16, 8>);       \
+  else                                                                 \
+    G2_KERNEL(4, attention_paged_matrix_kernel<E, CPL, P16, 4>);
+#define G2_ROWS(LPR)                                                   \
+  if (p.waves == 8 && p.gq == 1)                                       \
+    G2_KERNEL(8, attention_paged_kernel<E, LPR, 1, 4, 8, false>);      \
+  else if (p.waves == 8)                                               \
+    G2_KERNEL(8, attention_paged_kernel<E, LPR, 2, 4, 8, false>);      \
+  else if (p.gq == 1)                                                  \
+    G2_KERNEL(4, attention_paged_kernel<E, LPR, 1, 8, 4, false>);      \
+  else                                                                 \
+    G2_KERNEL(4, attention_paged_kernel<E, LPR, 2, 4, 4, false>);
+  if (p.matrix && HS <= 64) {
+    G2_MATRIX(4, (sizeof(E) == 4 ? 2 : 4))
+  } else if (p.matrix && HS <= 128) {
+    G2_MATRIX(8, (sizeof(E) == 4 ? 1 : 2))
+  } else if (p.matrix) {
+    G2_KERNEL(4, attention_paged_matrix_kernel<E, 16, 1, 4>);
+  } else if (!p.rows16) {
+    if (p.gq == 1)
+      G2_KERNEL(4, attention_paged_kernel<E, 64, 1, 8, 4, true>);
+    else if (p.gq == 2)
+      G2_KERNEL(4, attention_paged_kernel<E, 64, 2, 8, 4, true>);
+    else
+      G2_KERNEL(4, attention_paged_kernel<E, 64, 4, 4, 4, true>);
+  } else if (lanes <= 8) {
+    G2_ROWS(8)
+  } else if (lanes <= 16) {
+    G2_ROWS(16)
+  } else if (lanes <= 32) {
+    G2_ROWS(32)
+  } else if constexpr (sizeof(E) == 4) {
+    G2_ROWS(64)
+  }
+#undef G2_ROWS
+#undef G2_MATRIX
+#undef G2_KERNEL
 }
 
 }  // namespace g2
@@ -750,8 +1480,8 @@ size_t attention_decode_paged_workspace(const GPT2PagedCache* cache, int B, int 
   Pages pg;
   if (check_cache("attention_decode_paged_workspace", cache, pg)) return 0;
   if (B < 1 || NH < 1 || NH % pg.kv_heads != 0) return 0;
-  const int S = ranges_for(B, pg.kv_heads, NH / pg.kv_heads, pg.capacity);
-  return part_bytes(B, NH, pg.head_size, S) + (weights ? score_bytes(B, NH, pg.capacity) : 0);
+  const AttendSpace space(B, NH, (pg.head_size + 3) & ~3, (pg.capacity + 63) & ~63, plan_attend(cache, B, NH).S, weights);
+  return GPT2HIP_PAGED_COUNTER_BYTES + space.total * sizeof(float);
 }
 
 int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const float* inp, int inp_stride,
@@ -772,6 +1502,7 @@ int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const
   if (!out || !inp || !lengths) return fail(GPT2HIP_EINVAL, "attention_decode_paged: null pointer");
   if ((uintptr_t)workspace % 256) return fail(GPT2HIP_EINVAL, "attention_decode_paged: workspace must be 256-byte aligned");
   const bool weights = weights_out != nullptr;
+  AttendPlan plan = plan_attend(cache, B, NH);
   a.out = out;
   a.inp = inp;
   a.lengths = lengths;
@@ -780,41 +1511,43 @@ int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const
   a.B = B;
   a.NH = NH;
   a.G = NH / KVH;
-  const int gq = heads_at_once(a.G);
-  a.chunks = (a.G + gq - 1) / gq;
+  a.chunks = plan.chunks;
   a.stride = inp_stride;
   a.append = append ? 1 : 0;
+  a.part_stride = (HS + 3) & ~3;
+  a.score_stride = (a.pg.capacity + 63) & ~63;
   a.scale_log2e = (1.0f / sqrtf((float)HS)) * 1.4426950408889634f;
-  // as many ranges as the workspace holds, behind the scores
-  const size_t scores = weights ? score_bytes(B, NH, a.pg.capacity) : 0;
-  if (!workspace) workspace_bytes = 0;
-  a.S = ranges_for(B, KVH, a.G, a.pg.capacity);
-  const size_t one = part_bytes(B, NH, HS, 1);
-  const size_t room = workspace_bytes > scores ? (workspace_bytes - scores) / one : 0;
-  if (weights && room < 1)
-    return fail(GPT2HIP_EINVAL, "attention_decode_paged: weights need a workspace of at least %zu bytes, got %zu", scores + one,
-                workspace_bytes);
-  if (room < (size_t)a.S) a.S = room < 1 ? 1 : (int)room;
-  const bool parts = a.S > 1 || weights;
-  float* at = (float*)workspace;
-  a.part_o = parts ? at : nullptr;
-  a.part_ml = parts ? at + (size_t)B * NH * a.S * HS : nullptr;
-  a.scores = weights ? a.part_ml + (size_t)B * NH * a.S * 2 : nullptr;
+  // as many ranges as the workspace holds
+  const size_t room = workspace && workspace_bytes > GPT2HIP_PAGED_COUNTER_BYTES
+                          ? (workspace_bytes - GPT2HIP_PAGED_COUNTER_BYTES) / sizeof(float) : 0;
+  auto space = [&](int S) { return AttendSpace(B, NH, a.part_stride, a.score_stride, S, weights); };
+  while (plan.S > 1 && space(plan.S).total > room) plan.S--;
+  const AttendSpace use = space(plan.S);
+  if (use.total > room)
+    return fail(GPT2HIP_EINVAL, "attention_decode_paged: weights need a workspace of at least %zu bytes, got %zu",
+                GPT2HIP_PAGED_COUNTER_BYTES + use.total * sizeof(float), workspace_bytes);
+  a.S = plan.S;
+  a.min_range = plan.min_range;
+  a.counters = (unsigned*)workspace;
+  float* at = workspace ? (float*)((char*)workspace + GPT2HIP_PAGED_COUNTER_BYTES) : nullptr;
+  a.part_o = at;
+  a.part_ml = at + use.ml;
+  a.joined = weights ? at + use.joined : nullptr;
+  a.scores = weights ? at + use.scores : nullptr;
+  a.weigh_here = weights && a.S == 1 && a.chunks == 1;
   const long long blocks = (long long)B * KVH * a.chunks * a.S;
-  const long long joins = (long long)B * NH +
-      (weights ? (long long)B * KVH * ((a.pg.capacity + kJoinPositions - 1) / kJoinPositions) : 0);
-  if (blocks > 0x7fffffffLL || joins > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "attention_decode_paged: grid too large");
-  const bool vec = rows_by_16(cache);
+  const long long weighs = (long long)B * KVH * ((a.pg.capacity + kWeighPositions - 1) / kWeighPositions);
+  if (blocks > 0x7fffffffLL || weighs > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "attention_decode_paged: grid too large");
   if (cache->type == GPT2HIP_F32)
-    launch_attend<float>(a, (unsigned)blocks, vec);
+    launch_attend<float>(a, plan, (unsigned)blocks);
   else if (cache->type == GPT2HIP_F16)
-    launch_attend<f16>(a, (unsigned)blocks, vec);
+    launch_attend<f16>(a, plan, (unsigned)blocks);
   else
-    launch_attend<bf16>(a, (unsigned)blocks, vec);
+    launch_attend<bf16>(a, plan, (unsigned)blocks);
   G2_LAUNCH_CHECK("attention_decode_paged");
-  if (parts) {
-    hipLaunchKernelGGL(attention_paged_join_kernel, dim3((unsigned)joins), dim3(256), 0, stream(), a);
-    G2_LAUNCH_CHECK("attention_decode_paged (join)");
+  if (weights && !a.weigh_here) {
+    hipLaunchKernelGGL(attention_paged_weights_kernel, dim3((unsigned)weighs), dim3(kWeighPositions), 0, stream(), a);
+    G2_LAUNCH_CHECK("attention_decode_paged (weights)");
   }
   return GPT2HIP_OK;
 }
@@ -844,21 +1577,22 @@ int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, 
   const int groups = (budget + 63) / 64;
   const long long pairs = (long long)B * KVH, blocks = (pairs * groups + 3) / 4;
   if (pairs > 0x7fffffffLL || blocks > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "kv_evict_paged: grid too large");
-  const dim3 picks((unsigned)pairs), pick_block(kPickWaves * kWave);
   const int most = from.capacity - recent;  // weights that can take part
-#define G2_PICK(R)                                                                                              \
-  hipLaunchKernelGGL((kv_evict_pick_kernel<R>), picks, pick_block, 0, stream(), kept, lengths_out, weights_in,   \
-                     lengths, KVH, from.capacity, budget, recent)
-  if (most <= 1024)
-    G2_PICK(1);
+#define G2_PICK(WAVES, R)                                                                                   \
+  hipLaunchKernelGGL((kv_evict_pick_kernel<WAVES, R>), dim3((unsigned)pairs), dim3(WAVES * kWave), 0, stream(), kept, \
+                     lengths_out, weights_in, lengths, KVH, from.capacity, budget, recent)
+  if (most <= 256)
+    G2_PICK(4, 1);
+  else if (most <= 1024)
+    G2_PICK(4, 4);
   else if (most <= 4 * 1024)
-    G2_PICK(4);
+    G2_PICK(16, 4);
   else if (most <= 16 * 1024)
-    G2_PICK(16);
+    G2_PICK(16, 16);
   else if (most <= 32 * 1024)
-    G2_PICK(32);
+    G2_PICK(16, 32);
   else
-    G2_PICK(0);
+    G2_PICK(16, 0);
 #undef G2_PICK
   G2_LAUNCH_CHECK("kv_evict_paged (choice)");
   const int row_bytes = (int)(from.head_size * type_bytes(src->type));

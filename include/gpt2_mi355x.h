@@ -266,8 +266,12 @@ int kv_store_paged_status(const GPT2PagedCache* cache, const float* inp, int inp
  * workspace: device memory, 256-byte aligned, for the work to be split over the cache's length;
  * attention_decode_paged_workspace gives the bytes that never constrain the split (0: bad
  * arguments).  With less the work is split less, NULL / 0 means not at all, but weights need
- * what holds B * NH * (max_pages * page_size + head_size + 2) floats.  Its contents do not
- * matter before and mean nothing after; calls that overlap on one GPU need a workspace each. */
+ * GPT2HIP_PAGED_COUNTER_BYTES and B * NH * (max_pages * page_size + 68) floats.  Its first
+ * GPT2HIP_PAGED_COUNTER_BYTES are counters: zero them once (hipMemset) before the first call;
+ * every call leaves them zero (zero them again after a launch that did not run to completion).
+ * The rest is scratch.  Calls that overlap on one GPU need a workspace each, calls of any sizes
+ * one after the other can share one. */
+#define GPT2HIP_PAGED_COUNTER_BYTES 65536u
 size_t attention_decode_paged_workspace(const GPT2PagedCache* cache, int B, int NH, int weights);
 int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const float* inp, int inp_stride,
                                   const int* lengths, const float* weights_in, float* weights_out, int B, int NH,

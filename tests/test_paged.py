@@ -74,8 +74,8 @@ def test_attend_refusals():
     for k in ("out", "inp", "lengths"):
         assert attend(c, **{k: None}) == 1 and b"null" in message()
     assert attend(c, ws=FAKE + 64, nbytes=1 << 20) == 1 and b"256-byte" in message()
-    # weights need room for the scores and one range
-    least = 2 * 4 * (64 + 64 + 2) * 4
+    # weights need room for the counters, the scores and the rows' maxima and sums
+    least = g2.PAGED_COUNTER_BYTES + 2 * 4 * (64 + 2) * 4
     assert attend(c, win=FAKE, wout=FAKE) == 1 and str(least).encode() in message()
     assert attend(c, win=FAKE, wout=FAKE, ws=FAKE, nbytes=least - 1) == 1
     assert attend(c, B=0, out=None, inp=None) == 0
@@ -87,9 +87,9 @@ def test_workspace_size():
     p = ctypes.addressof(c)
     assert f(p, 0, 4, 0) == 0 and f(p, 2, 3, 0) == 0 and f(None, 2, 4, 0) == 0
     plain, scored = f(p, 2, 4, 0), f(p, 2, 4, 1)
-    assert plain % (2 * 4 * 66 * 4) == 0 and scored - plain == 2 * 4 * 1024 * 4
+    assert g2.PAGED_COUNTER_BYTES < plain and scored - plain == 2 * 4 * (1024 + 2) * 4
     # many sequences need no split, few long ones do
-    assert f(p, 2000, 4, 0) < 2000 * 4 * 66 * 4 * 3 and f(p, 1, 4, 0) >= 1 * 4 * 66 * 4 * 8
+    assert f(p, 4000, 4, 0) == g2.PAGED_COUNTER_BYTES and f(p, 1, 4, 0) >= g2.PAGED_COUNTER_BYTES + 4 * 66 * 4 * 4
 
 
 def test_evict_refusals():

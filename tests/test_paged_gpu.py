@@ -123,9 +123,10 @@ def check_attend(c, append=True, weights=False, workspace="full", view=False, ca
     ws = None
     if workspace == "full":
         ws = g2.attention_decode_paged_workspace(cache, B, NH, weights=weights)
-        ws.fill_(0xFF)  # NaN everywhere
     elif workspace:
-        ws = torch.full((workspace,), 0xFF, dtype=torch.uint8, device="cuda")
+        ws = torch.zeros(workspace, dtype=torch.uint8, device="cuda")
+    if ws is not None:
+        ws[g2.PAGED_COUNTER_BYTES:] = 0xFF  # NaN everywhere behind the counters
     w = wo = None
     if weights:
         w = torch.rand((B, KVH, c.cap), generator=c.g).cuda() * 3
@@ -133,6 +134,7 @@ def check_attend(c, append=True, weights=False, workspace="full", view=False, ca
     for _ in range(calls):
         g2.attention_decode_paged(out, cache, inp, c.dl, B, NH, append=append, weights_in=w, weights_out=wo, workspace=ws)
     torch.cuda.synchronize()
+    assert ws is None or (ws[: g2.PAGED_COUNTER_BYTES] == 0).all(), "a counter was left behind"
     assert (flat[:pad] == 7).all() and (flat[-pad:] == 7).all(), "write outside the output"
     want_k, want_v = c.keys.clone(), c.values.clone()
     for b, n in enumerate(c.lengths):
@@ -174,7 +176,7 @@ def check_attend(c, append=True, weights=False, workspace="full", view=False, ca
 
 SHAPES = [  # NH, KVH, HS
     (12, 12, 64), (25, 25, 64), (8, 2, 128), (32, 4, 96), (6, 3, 80), (7, 1, 64), (3, 3, 256), (9, 3, 32), (10, 5, 16),
-    (2, 1, 8), (16, 1, 64),
+    (2, 1, 8), (16, 1, 64), (12, 1, 64), (40, 2, 128), (24, 2, 256), (18, 6, 72), (4, 1, 136), (15, 5, 8),
 ]
 
 
@@ -250,7 +252,7 @@ def test_attend_split_as_far_as_the_workspace_goes():
     """None, room for one range, for three, and the full size: the same row to rounding each time."""
     lengths = [4000, 1, 2500]
     one = 3 * 4 * (64 + 2) * 4
-    for ws in (None, 256, one, 3 * one + 100, "full"):
+    for ws in (None, 256, g2.PAGED_COUNTER_BYTES, g2.PAGED_COUNTER_BYTES + one, g2.PAGED_COUNTER_BYTES + 3 * one + 100, "full"):
         say(f"workspace {ws}")
         check_attend(Case(9, "f32", 3, 4, 4, 64, 32, lengths, 4001), workspace=ws)
 
@@ -260,32 +262,42 @@ def test_attend_rows_at_a_stride():
     check_attend(Case(11, "f32", 5, 6, 2, 64, 16, [0, 17, 200, -1, 500], 512), view=True, append=False)
 
 
-def test_attend_large_scores():
+@pytest.mark.parametrize("kind,NH", [("f32", 2), ("f32", 8), ("f16", 8), ("bf16", 8)])
+def test_attend_large_scores(kind, NH):
     """Scores of some hundreds: one position has all the weight, exp must neither overflow nor lose it."""
-    c = Case(12, "f32", 2, 2, 2, 64, 16, [300, 700], 701, keys_std=60.0)
-    check_attend(c, weights=True)
+    check_attend(Case(12, kind, 2, NH, 2, 64, 16, [300, 700], 701, keys_std=60.0), weights=True)
 
 
-def test_attend_infinite_keys_weigh_nothing():
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("scale", [1e-12, 1e-3, 1e4])
+def test_attend_queries_of_any_size(kind, scale):
+    """Queries far below and above 1, keys that make up for it: pieces of queries lose nothing."""
+    c = Case(19, kind, 2, 8, 2, 64, 16, [300, 700], 701, keys_std=min(1 / scale, 1e3) if kind != "f16" else 1.0)
+    c.inp[:, : 8 * 64] *= scale
+    c.inp[0, 64:128] *= torch.logspace(-6, 0, 64)
+    check_attend(c)
+
+
+@pytest.mark.parametrize("kind,NH", [("f32", 1), ("f16", 1), ("bf16", 2), ("f32", 5), ("f16", 5), ("bf16", 5), ("bf16", 16)])
+def test_attend_infinite_keys_weigh_nothing(kind, NH):
     """Positions whose score is -inf (a key with an infinity against a negative query) weigh nothing,
     even when they are all that a row group, a wave or a range has seen."""
+    say(f"infinite keys {kind} NH={NH}")
     n = 900
-    c = Case(13, "f32", 1, 1, 1, 64, 16, [n], n + 1)
-    c.inp[0, 0] = -1.0
+    c = Case(13, kind, 1, NH, 1, 64, 16, [n], n + 1)
+    c.inp[0, : NH * 64: 64] = -1.0
     live = [5, 640]
     for i in range(n):
         if i not in live:
             c.keys[c.table[0, i // 16], 0, i % 16] = 0.0
             c.keys[c.table[0, i // 16], 0, i % 16, 0] = float("inf")
-            c.k64[0][0, i] = 0.0
-            c.k64[0][0, i, 0] = float("inf")
     cache = c.gpu()
-    out = torch.zeros((1, 64), device="cuda")
-    for ws in (None, g2.attention_decode_paged_workspace(cache, 1, 1)):
-        g2.attention_decode_paged(out, cache, c.inp.cuda(), c.dl, 1, 1, workspace=ws)
+    out = torch.zeros((1, NH * 64), device="cuda")
+    for ws in (None, g2.attention_decode_paged_workspace(cache, 1, NH)):
+        g2.attention_decode_paged(out, cache, c.inp.cuda(), c.dl, 1, NH, workspace=ws)
         k, v = c.rows(0, True)
         rows = live + [n]
-        q, k, v = c.inp[0, :64].double().view(1, 1, 64), k[:, rows], v[:, rows]
+        q, k, v = c.inp[0, : NH * 64].double().view(1, NH, 64), k[:, rows], v[:, rows]
         s = torch.matmul(q, k.transpose(1, 2)) / 8.0
         p = torch.softmax(s, -1)
         tol, _ = attention_bound(q, k, v, p, s)
