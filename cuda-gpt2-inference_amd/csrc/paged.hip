@@ -9,13 +9,6 @@
 
 #include "common.hpp"
 
-#ifndef G2_MATRIX_FROM
-#define G2_MATRIX_FROM 3
-#endif
-#ifndef G2_RANGE_BYTES
-#define G2_RANGE_BYTES 65536
-#endif
-
 namespace g2 {
 
 typedef _Float16 f16;
@@ -136,11 +129,16 @@ __global__ __launch_bounds__(256) void kv_store_paged_kernel(Pages pg, const flo
     const int head = c / HS, d = c - head * HS;
     E* to = (E*)(value ? pg.values : pg.keys) + ((size_t)row0 + (size_t)head * pg.divide.size) * HS + d;
     if constexpr (VEC == 4) {
+      typedef unsigned Words __attribute__((ext_vector_type(sizeof(E))));
       const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(src + i));
-      struct alignas(4 * sizeof(E)) Four {
+      struct Four {
         E e[4];
       };
-      *reinterpret_cast<Four*>(to) = Four{{narrow<E>(x[0]), narrow<E>(x[1]), narrow<E>(x[2]), narrow<E>(x[3])}};
+      const Words y = __builtin_bit_cast(Words, (Four{{narrow<E>(x[0]), narrow<E>(x[1]), narrow<E>(x[2]), narrow<E>(x[3])}}));
+      if constexpr (sizeof(E) == 2)
+        __builtin_nontemporal_store(y, reinterpret_cast<Words*>(to));
+      else
+        *reinterpret_cast<Words*>(to) = y;
     } else {
       to[0] = narrow<E>(src[i]);
     }
@@ -1100,18 +1098,38 @@ __device__ __forceinline__ int wave_sum_int(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);
   v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
   v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  const auto h = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  v = (int)(h[0] + h[1]);
+  const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  return (int)(r[0] + r[1]);
+}
+
+// base + the set bits of m in front of this lane's
+__device__ __forceinline__ int lanes_before(unsigned long long m, int base) {
+  return __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, base));
+}
+
+// The sum over WAVES consecutive lanes of a row of 16, in each of them.
+template <int WAVES>
+__device__ __forceinline__ int waves_sum(int v) {
+  static_assert(WAVES == 4 || WAVES == 16, "quads or rows");
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);
+  if constexpr (WAVES == 16) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
+  }
+  return v;
 }
 
 constexpr int kFew = 4096;  // ranks that are worth a list of their own
 
 // One workgroup per (sequence, kv head) chooses the positions that stay: the `recent` last ones
 // and, of the others, the budget - recent of largest weight.  The smallest rank that stays is
-// found two bits at a time by counting how many ranks reach each of three candidates: sums of
-// integers, the same on every run.  Once few ranks are left that could be it, they are listed in
+// found two bits at a time by counting how many ranks go each of the four ways: sums of integers,
+// the same on every run.  Once few ranks are left that could be it, they are listed in
 // LDS and the rest is not looked at again until the end; the search ends early where a candidate
-// is reached by exactly as many as are wanted.  A wave owns consecutive positions, so that the
+// is reached by exactly as many ranks as are wanted.  A wave owns consecutive positions, so that the
 // places in the output follow from counts alone.  R ranks per thread are kept in registers;
 // R = 0: any length, read again for every count.
 template <int WAVES, int R>
@@ -1122,11 +1140,10 @@ __global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
   constexpr bool LISTS = R == 0 || R * THREADS > 2 * kFew;
   constexpr int FEW = LISTS ? kFew / THREADS : 1;
   __shared__ unsigned list[LISTS ? kFew : 1];
-  __shared__ int counts[16][3], waves[2][WAVES], listed;
+  __shared__ int counts[2][WAVES][3], waves[2][WAVES], listed;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t bh = blockIdx.x;
   const int b = (int)(bh / KVH);
-  if (tid < 48) (&counts[0][0])[tid] = 0;
   if (tid == 0) listed = 0;
   const int n = lengths[b];
   if (n < 0) return;
@@ -1171,41 +1188,57 @@ __global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
   bool from_list = false;
   __syncthreads();
 
-  unsigned low = 0u;              // at least `want` ranks reach it ...
-  int reach = older, over = 0;    // ... this many; and this many are too large to be the one sought
-  int unlisted = 0;               // how many of those are not on the list
+  unsigned low = 0u;            // at least `want` ranks reach it ...
+  int reach = older, over = 0;  // ... this many; and this many are too large to be the one sought
   for (int step = 0; step < 16 && reach != want; step++) {
+    // the four ways the next two bits can go, for ranks that agree with low in front of them
     const int shift = 30 - 2 * step;
-    const unsigned t1 = low | (1u << shift), t2 = low | (2u << shift), t3 = low | (3u << shift);
-    int c1 = 0, c2 = 0, c3 = 0;
-    auto count = [&](unsigned x) {
-      c1 += x >= t1;
-      c2 += x >= t2;
-      c3 += x >= t3;
-    };
-    if (LISTS && from_list) {
+    int n1, n2, n3;
+    if (R > 0 || from_list) {
+      // four counts of 7 bits, and what is elsewhere runs out at the top
+      unsigned c = 0u;
+      auto count = [&](unsigned x) { c += 1u << (7u * min((x - low) >> shift, 4u)); };
+      if (LISTS && from_list) {
 #pragma unroll
-      for (int k = 0; k < FEW; k++) count(few[k]);
+        for (int k = 0; k < FEW; k++) count(few[k]);
+      } else {
+        each([&](int, unsigned x) { count(x); });
+      }
+      n1 = wave_sum_int((c >> 7) & 127u);
+      n2 = wave_sum_int(((c >> 14) & 127u) | ((c >> 21) & 127u) << 16);
+      n3 = n2 >> 16;
+      n2 &= 0xffff;
     } else {
-      each([&](int, unsigned x) { count(x); });
+      n1 = n2 = n3 = 0;
+      each([&](int, unsigned x) {
+        const unsigned d = (x - low) >> shift;
+        n1 += d == 1u;
+        n2 += d == 2u;
+        n3 += d == 3u;
+      });
+      n1 = wave_sum_int(n1);
+      n2 = wave_sum_int(n2);
+      n3 = wave_sum_int(n3);
     }
-    c1 = wave_sum_int(c1);
-    c2 = wave_sum_int(c2);
-    c3 = wave_sum_int(c3);
-    if (lane < 3) atomicAdd(&counts[step][lane], lane == 0 ? c1 : lane == 1 ? c2 : c3);
-    __syncthreads();
-    c1 = counts[step][0] + unlisted;
-    c2 = counts[step][1] + unlisted;
-    c3 = counts[step][2] + unlisted;
+    if (lane == 0) {
+      counts[step & 1][wave][0] = n1;
+      counts[step & 1][wave][1] = n2;
+      counts[step & 1][wave][2] = n3;
+    }
+    __syncthreads();  // the counts of the step before last have been read by then
+    n1 = waves_sum<WAVES>(counts[step & 1][lane & (WAVES - 1)][0]);
+    n2 = waves_sum<WAVES>(counts[step & 1][lane & (WAVES - 1)][1]);
+    n3 = waves_sum<WAVES>(counts[step & 1][lane & (WAVES - 1)][2]);
+    const int c3 = over + n3, c2 = c3 + n2, c1 = c2 + n1;
     if (c3 >= want) {
-      low = t3;
+      low |= 3u << shift;
       reach = c3;
     } else if (c2 >= want) {
-      low = t2;
+      low |= 2u << shift;
       reach = c2;
       over = c3;
     } else if (c1 >= want) {
-      low = t1;
+      low |= 1u << shift;
       reach = c1;
       over = c2;
     } else {
@@ -1213,35 +1246,38 @@ __global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
     }
     if constexpr (LISTS) {
       if (!from_list && reach - over <= kFew && reach != want) {
+        int mine = 0;
+        each([&](int, unsigned x) { mine += x != 0u && (x - low) >> shift == 0u; });
+        mine = wave_sum_int(mine);
+        if (lane == 0) mine = atomicAdd(&listed, mine);
+        int at = __builtin_amdgcn_readfirstlane(mine);
         each([&](int, unsigned x) {
-          const bool in = x >= low && x - low < (1u << shift);
+          const bool in = x != 0u && (x - low) >> shift == 0u;
           const unsigned long long m = __ballot(in);
-          if (m) {
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&listed, __popcll(m));
-            at = __shfl(at, 0, 64) + __popcll(m & ((1ull << lane) - 1ull));
-            if (in) list[at] = x;
-          }
+          const int to = lanes_before(m, at);
+          if (in && to < kFew) list[to] = x;
+          at += __popcll(m);
         });
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < FEW; k++) few[k] = k * THREADS + tid < listed ? list[k * THREADS + tid] : 0u;
+        for (int k = 0; k < FEW; k++) few[k] = k * THREADS + tid < min(listed, kFew) ? list[k * THREADS + tid] : 0u;
         from_list = true;
-        unlisted = over;
       }
     }
   }
 
-  // all ranks above low stay, and of its equals as many as there is room for
+  // All ranks above low stay, and of its equals as many as there is room for: all of them, where
+  // exactly as many as are wanted reach low.
+  const bool exact = reach == want;
   int gt = 0, eq = 0;
   each([&](int, unsigned x) {
-    gt += x > low;
+    gt += x >= low;
     eq += x == low;
   });
   gt = wave_sum_int(gt);
   eq = wave_sum_int(eq);
   if (lane == 0) {
-    waves[0][wave] = gt;
+    waves[0][wave] = exact ? gt : gt - eq;
     waves[1][wave] = eq;
   }
   __syncthreads();
@@ -1252,63 +1288,88 @@ __global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
     gt_before += i < wave ? waves[0][i] : 0;
     eq_before += i < wave ? waves[1][i] : 0;
   }
+  if (exact) {
+    each([&](int r, unsigned x) {
+      const unsigned long long g = __ballot(x >= low);
+      const int at = lanes_before(g, gt_before);
+      if (x >= low && at < want) out[at] = first + r * 64 + lane;
+      gt_before += __popcll(g);
+    });
+    return;
+  }
   const int room = want - above_all;  // the lowest positions have it
-  const unsigned long long before = (1ull << lane) - 1ull;
   each([&](int r, unsigned x) {
     const unsigned long long g = __ballot(x > low), e = __ballot(x == low);
-    const int eq_at = eq_before + __popcll(e & before);
-    const int at = gt_before + __popcll(g & before) + min(eq_at, room);
+    const int eq_at = lanes_before(e, eq_before), at = lanes_before(g, gt_before) + min(eq_at, room);
     if ((x > low || (x == low && eq_at < room)) && at < want) out[at] = first + r * 64 + lane;
     gt_before += __popcll(g);
     eq_before += __popcll(e);
   });
 }
 
-// Copies what stays into the pages of the other table: a wave moves the keys and values of ROWS
-// rows of one (sequence, kv head), 16 bytes per lane, and their weights.
-template <int UNIT>  // bytes per lane and load: 16, or the size of an element
+// Copies what stays into the pages of the other table.  A wave moves the keys and values of
+// kCopyLoads times as many rows of one (sequence, kv head) as one load of it holds, all loads
+// ahead of the stores, and their weights.  UNIT: bytes per lane and load, 16 or the size of an
+// element.
+constexpr int kCopyLoads = 4;
+static int copy_rows(int row_bytes, int unit) {  // rows per wave
+  const int units = row_bytes / unit, per = units < 64 ? 64 / units : 1;
+  return per * kCopyLoads < 64 ? per * kCopyLoads : 64;
+}
+template <int UNIT, bool STREAM>
 __global__ __launch_bounds__(256) void kv_evict_copy_kernel(Pages dst, Pages src, const int* __restrict__ kept,
                                                             float* __restrict__ weights_out,
                                                             const float* __restrict__ weights_in,
                                                             const int* __restrict__ lengths, int B, int budget,
-                                                            int row_bytes, int groups) {
+                                                            int row_bytes, int rows, int groups) {
   const int lane = threadIdx.x & 63;
   const size_t id = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int KVH = src.kv_heads;
   const size_t bh = id / groups;
   const int b = (int)(bh / KVH), h = (int)(bh % KVH);
   if (b >= B) return;
+  const int j0 = (int)(id % groups) * rows, j = j0 + lane;
   const int n = lengths[b];
   if (n < 0 || n > src.capacity) return;
-  const int j0 = (int)(id % groups) * 64, stay = min(n, budget);
+  const int stay = min(n, budget);
   if (j0 >= stay) return;
-  const int j = j0 + lane;
   unsigned from = 0, to = 0;
-  bool ok = j < stay;
+  bool ok = lane < rows && j < stay;
   if (ok) {
-    const int i = kept[bh * budget + j];
-    from = src.row(b, h, min(max(i, 0), n - 1), ok);
+    const int i = min(max(kept[bh * budget + j], 0), n - 1);
+    const float w = weights_in[bh * src.capacity + i];
+    from = src.row(b, h, i, ok);
     to = dst.row(b, h, j, ok);
-    weights_out[bh * dst.capacity + j] = ok ? weights_in[bh * src.capacity + min(max(i, 0), n - 1)] : __builtin_nanf("");
+    weights_out[bh * dst.capacity + j] = ok ? w : __builtin_nanf("");
   }
   const unsigned long long live = __ballot(ok);
-  const int units = row_bytes / UNIT, per = 64 / units > 0 ? 64 / units : 1;  // rows per load
-  for (int r = 0; r < 64; r += per) {
-    const int mine = r + lane / units;
-    const unsigned f = __shfl(from, mine & 63, 64), t = __shfl(to, mine & 63, 64);
-    if (mine >= 64 || mine >= r + per || !((live >> (mine & 63)) & 1ull)) continue;
-    for (int c = lane % units; c < units; c += 64) {
-      const size_t x = (size_t)f * row_bytes + (size_t)c * UNIT, y = (size_t)t * row_bytes + (size_t)c * UNIT;
-      if constexpr (UNIT == 16) {
-        const u32x4 kk = __builtin_nontemporal_load((const u32x4*)((const char*)src.keys + x));
-        const u32x4 vv = __builtin_nontemporal_load((const u32x4*)((const char*)src.values + x));
-        __builtin_nontemporal_store(kk, (u32x4*)((char*)dst.keys + y));
-        __builtin_nontemporal_store(vv, (u32x4*)((char*)dst.values + y));
-      } else {
-        typedef typename std::conditional<UNIT == 4, unsigned, unsigned short>::type W;
-        const W kk = *(const W*)((const char*)src.keys + x), vv = *(const W*)((const char*)src.values + x);
-        *(W*)((char*)dst.keys + y) = kk;
-        *(W*)((char*)dst.values + y) = vv;
+  const int units = row_bytes / UNIT, per = units < 64 ? 64 / units : 1;  // units per row, rows per load
+  const int mine = lane / units;
+  typedef typename std::conditional<UNIT == 16, u32x4, typename std::conditional<UNIT == 4, unsigned, unsigned short>::type>::type Word;
+  const Word *ks = (const Word*)src.keys, *vs = (const Word*)src.values;
+  Word *kd = (Word*)dst.keys, *vd = (Word*)dst.values;
+  const int c0 = lane - mine * units;  // a row of more than 64 units takes more than one round, all lanes in each
+  for (int round = 0; round < units; round += 64) {
+    const int c = min(c0 + round, units - 1);
+    Word k[kCopyLoads], v[kCopyLoads];
+#pragma unroll
+    for (int u = 0; u < kCopyLoads; u++) {
+      const size_t x = (size_t)__shfl(from, (u * per + mine) & 63, 64) * units + c;  // row 0 where there is none
+      k[u] = __builtin_nontemporal_load(ks + x);
+      v[u] = __builtin_nontemporal_load(vs + x);
+    }
+#pragma unroll
+    for (int u = 0; u < kCopyLoads; u++) {
+      const int r = u * per + mine;
+      const size_t x = (size_t)__shfl(to, r & 63, 64) * units + c;
+      if (mine < per && r < rows && c0 + round < units && ((live >> (r & 63)) & 1ull)) {
+        if constexpr (STREAM) {
+          __builtin_nontemporal_store(k[u], kd + x);
+          __builtin_nontemporal_store(v[u], vd + x);
+        } else {
+          kd[x] = k[u];
+          vd[x] = v[u];
+        }
       }
     }
   }
@@ -1370,7 +1431,7 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
   AttendPlan p;
   const int G = NH / c->kv_heads;
   p.rows16 = rows_by_16(c);
-  p.matrix = p.rows16 && G >= G2_MATRIX_FROM;
+  p.matrix = p.rows16 && G >= 3;
   p.gq = p.matrix ? kMatrixHeads : G >= 3 ? 4 : G;
   p.chunks = (G + p.gq - 1) / p.gq;
   const long long groups = (long long)B * c->kv_heads * p.chunks;
@@ -1380,7 +1441,7 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
   // One workgroup per compute unit, or two where each has enough to do: the longest sequence's
   // workgroups must not outlast the others'.  A range is worth a workgroup from 64 KB on.
   const long long row_bytes = 2LL * c->head_size * type_bytes(c->type), capacity = (long long)c->max_pages * c->page_size;
-  p.min_range = (int)((G2_RANGE_BYTES / row_bytes + 63) & ~63LL);
+  p.min_range = (int)((65536 / row_bytes + 63) & ~63LL);
   if (p.min_range < 128) p.min_range = 128;
   long long S = 512 / groups;
   if (S < 1 || capacity * row_bytes / S < 512 * 1024) S = 256 / groups;
@@ -1574,7 +1635,9 @@ int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, 
   if (weights_out == weights_in || lengths_out == lengths)
     return fail(GPT2HIP_EINVAL, "kv_evict_paged: weights_out and lengths_out must not be the inputs");
   const int KVH = from.kv_heads;
-  const int groups = (budget + 63) / 64;
+  const int row_bytes = (int)(from.head_size * type_bytes(src->type));
+  const int unit = rows_by_16(src) && rows_by_16(dst) ? 16 : (int)type_bytes(src->type);
+  const int rows = copy_rows(row_bytes, unit), groups = (budget + rows - 1) / rows;
   const long long pairs = (long long)B * KVH, blocks = (pairs * groups + 3) / 4;
   if (pairs > 0x7fffffffLL || blocks > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "kv_evict_paged: grid too large");
   const int most = from.capacity - recent;  // weights that can take part
@@ -1595,17 +1658,18 @@ int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, 
     G2_PICK(16, 0);
 #undef G2_PICK
   G2_LAUNCH_CHECK("kv_evict_paged (choice)");
-  const int row_bytes = (int)(from.head_size * type_bytes(src->type));
   const dim3 grid((unsigned)blocks), block(256);
-#define G2_COPY(UNIT)                                                                                             \
-  hipLaunchKernelGGL((kv_evict_copy_kernel<UNIT>), grid, block, 0, stream(), to, from, kept, weights_out, weights_in, \
-                     lengths, B, budget, row_bytes, groups)
-  if (rows_by_16(src) && rows_by_16(dst))
-    G2_COPY(16);
-  else if (src->type == GPT2HIP_F32)
-    G2_COPY(4);
+#define G2_COPY(UNIT, STREAM)                                                                                             \
+  hipLaunchKernelGGL((kv_evict_copy_kernel<UNIT, STREAM>), grid, block, 0, stream(), to, from, kept, weights_out, weights_in, \
+                     lengths, B, budget, row_bytes, rows, groups)
+  if (unit == 16 && row_bytes % 128 == 0)  // whole cache lines
+    G2_COPY(16, true);
+  else if (unit == 16)
+    G2_COPY(16, false);
+  else if (unit == 4)
+    G2_COPY(4, false);
   else
-    G2_COPY(2);
+    G2_COPY(2, false);
 #undef G2_COPY
   G2_LAUNCH_CHECK("kv_evict_paged (copy)");
   return GPT2HIP_OK;

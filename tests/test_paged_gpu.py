@@ -591,6 +591,24 @@ def test_evict_ties_and_special_weights(weights, budget, recent):
     check_evict(budget, "f32", [300, 299, 256], budget, recent, max_len=320, weights=weights, HS=16)
 
 
+def negative(B, KVH, cap, g):
+    """Nothing but large negative weights: the smallest ranks there are."""
+    return -torch.rand((B, KVH, cap), generator=g) * 3e38
+
+
+@pytest.mark.parametrize("n,budget", [(300, 100), (9001, 8000), (20000, 19000), (20000, 40)])
+def test_evict_negative_weights(n, budget):
+    check_evict(8, "f32", [n, n - 7], budget, 10, KVH=1, HS=8, page=64, weights=negative)
+
+
+def test_evict_one_value_apart():
+    """Weights that differ in their last bits only."""
+    def close(B, KVH, cap, g):
+        return (torch.randint(0, 40, (B, KVH, cap), generator=g) + 0x3F800000).to(torch.int32).view(torch.float32)
+    for n, budget in ((900, 400), (9001, 4000), (30000, 7000)):
+        check_evict(9, "f16", [n, n - 3], budget, 0, KVH=1, HS=8, page=64, weights=close)
+
+
 def test_evict_ties_beyond_the_registers():
     check_evict(4, "f16", [40000, 39999], 20000, 100, KVH=1, HS=8, page=64, weights=ties)
 
