@@ -382,10 +382,10 @@ class PagedCache:
     float16 or bfloat16; table: contiguous int32 CUDA tensor (B, max_pages), the pages of each
     sequence in order.  The tensors are kept alive and used in place."""
 
-    _TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}  # GPT2HIP_F32, _F16, _BF16
-
     def __init__(self, keys, values, table):
-        if str(keys.dtype) not in self._TYPES or keys.dtype != values.dtype:
+        import torch
+        types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # GPT2HIP_F32, _F16, _BF16
+        if keys.dtype not in types or keys.dtype != values.dtype:
             raise TypeError(f"keys and values are float32, float16 or bfloat16 alike, got {keys.dtype}, {values.dtype}")
         if keys.dim() != 4 or keys.shape != values.shape:
             raise ValueError("keys and values are (num_pages, kv_heads, page_size, head_size) alike, got "
@@ -394,40 +394,46 @@ class PagedCache:
             raise ValueError(f"table is (B, max_pages), got {tuple(table.shape)}")
         self.keys, self.values, self.table = keys, values, table
         pages, heads, size, channels = keys.shape
-        self._c = GPT2PagedCache(_ptr(keys), _ptr(values), _i32(table), self._TYPES[str(keys.dtype)], pages,
-                                 size, table.shape[1], heads, channels)
+        self._c = GPT2PagedCache(_ptr(keys), _ptr(values), _i32(table), types[keys.dtype], pages, size,
+                                 table.shape[1], heads, channels)
         self.sequences, self.kv_heads, self.head_size = table.shape[0], heads, channels
         self.page_size, self.capacity = size, size * table.shape[1]  # capacity: positions per sequence
         self._ref = ctypes.addressof(self._c)
+        self._float, self._int = torch.float32, torch.int32
 
 
-def _has(t, what, *shape):
-    """Refuses a tensor of another shape than the library is going to assume."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what} is {shape}, got {tuple(t.shape)}")
+def _array(t, dtype, shape, what) -> int:
+    """Device pointer of a contiguous CUDA tensor of that type and shape."""
+    try:
+        if t.shape == shape and t.dtype is dtype and t.is_cuda and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    if not hasattr(t, "is_cuda") or not t.is_cuda or t.dtype is not dtype:
+        raise TypeError(f"{what} is a {dtype} CUDA tensor, got {getattr(t, 'dtype', type(t))} on "
+                        f"{getattr(t, 'device', 'the host')}")
+    raise ValueError(f"{what} is contiguous and {tuple(shape)}, got {tuple(t.shape)} with strides {t.stride()}")
 
 
-def _rows(inp, count, floats):
+def _rows(inp, count, floats, dtype):
     """(pointer, stride in floats) of `count` rows of at least `floats` floats; a view of a wider array will do."""
-    import torch
-    if not isinstance(inp, torch.Tensor) or not inp.is_cuda or inp.dtype != torch.float32:
+    if not hasattr(inp, "is_cuda") or not inp.is_cuda or inp.dtype is not dtype:
         raise TypeError("expected a float32 CUDA tensor of rows")
-    if inp.dim() != 2 or inp.shape[0] < count or inp.shape[1] < floats or (inp.shape[1] > 1 and inp.stride(1) != 1):
-        raise ValueError(f"expected {count} rows of {floats} consecutive floats, got {tuple(inp.shape)} "
-                         f"with strides {inp.stride()}")
+    shape, strides = inp.shape, inp.stride()
+    if len(shape) != 2 or shape[0] < count or shape[1] < floats or (shape[1] > 1 and strides[1] != 1):
+        raise ValueError(f"expected {count} rows of {floats} consecutive floats, got {tuple(shape)} with strides {strides}")
     # the stride of a single row says nothing
-    return inp.data_ptr(), inp.stride(0) if count > 1 else max(inp.stride(0), floats)
+    return inp.data_ptr(), strides[0] if count > 1 else max(strides[0], floats)
 
 
 def kv_store_paged(cache, inp, starts, lengths, N, B, NH):
     """Store the keys and values of N packed rows (q | k | v; NH = 0: k | v) into the pages: rows
     starts[b] .. starts[b + 1] - 1 become positions lengths[b] and on of sequence b."""
-    _has(lengths, "lengths", B)
-    _has(starts, "starts", B + 1)
     if B > cache.sequences:
         raise ValueError(f"the table lists {cache.sequences} sequences, asked for {B}")
-    rows, stride = _rows(inp, N, (NH + 2 * cache.kv_heads) * cache.head_size)
-    _check(lib().kv_store_paged_status(cache._ref, rows, stride, _i32(starts), _i32(lengths), N, B, NH), "kv_store_paged")
+    rows, stride = _rows(inp, N, (NH + 2 * cache.kv_heads) * cache.head_size, cache._float)
+    _check(lib().kv_store_paged_status(cache._ref, rows, stride, _array(starts, cache._int, (B + 1,), "starts"),
+                                       _array(lengths, cache._int, (B,), "lengths"), N, B, NH), "kv_store_paged")
 
 
 PAGED_COUNTER_BYTES = 65536  # GPT2HIP_PAGED_COUNTER_BYTES
@@ -449,32 +455,34 @@ def attention_decode_paged(out, cache, inp, lengths, B, NH, append=True, weights
     the new keys and values are stored as position lengths[b] first; otherwise inp holds queries
     that attend to the lengths[b] positions held.  weights_in, weights_out: accumulated attention
     weights (B, kv_heads, cache.capacity).  lengths[b] < 0: the row is left as it is."""
-    _has(lengths, "lengths", B)
-    _has(out, "out", B, NH * cache.head_size)
     if B > cache.sequences:
         raise ValueError(f"the table lists {cache.sequences} sequences, asked for {B}")
-    for what, w in (("weights_in", weights_in), ("weights_out", weights_out)):
-        if w is not None:
-            _has(w, what, B, cache.kv_heads, cache.capacity)
-    rows, stride = _rows(inp, B, (NH + (2 * cache.kv_heads if append else 0)) * cache.head_size)
-    ws, nbytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel() * workspace.element_size())
-    _check(lib().attention_decode_paged_status(_f32(out), cache._ref, rows, stride, _i32(lengths), _f32(weights_in),
-                                               _f32(weights_out), B, NH, int(append), ws, nbytes),
-           "attention_decode_paged")
+    f, HS = cache._float, cache.head_size
+    rows, stride = _rows(inp, B, (NH + 2 * cache.kv_heads if append else NH) * HS, f)
+    win = wout = ws = None
+    nbytes = 0
+    if weights_in is not None:
+        win = _array(weights_in, f, (B, cache.kv_heads, cache.capacity), "weights_in")
+    if weights_out is not None:
+        wout = _array(weights_out, f, (B, cache.kv_heads, cache.capacity), "weights_out")
+    if workspace is not None:
+        ws, nbytes = _ptr(workspace), workspace.nbytes
+    _check(lib().attention_decode_paged_status(_array(out, f, (B, NH * HS), "out"), cache._ref, rows, stride,
+                                               _array(lengths, cache._int, (B,), "lengths"), win, wout, B, NH,
+                                               1 if append else 0, ws, nbytes), "attention_decode_paged")
 
 
 def kv_evict_paged(dst, src, kept, weights_out, lengths_out, weights_in, lengths, B, budget, recent):
     """Bring every sequence down to `budget` positions (the `recent` last ones and the heaviest of the
     others, each kv head for itself), copied from the pages of src into those of dst."""
-    _has(lengths, "lengths", B)
-    _has(lengths_out, "lengths_out", B)
-    _has(kept, "kept", B, src.kv_heads, budget)
-    _has(weights_in, "weights_in", B, src.kv_heads, src.capacity)
-    _has(weights_out, "weights_out", B, dst.kv_heads, dst.capacity)
     if B > min(src.sequences, dst.sequences):
         raise ValueError(f"the tables list {src.sequences} and {dst.sequences} sequences, asked for {B}")
-    _check(lib().kv_evict_paged_status(dst._ref, src._ref, _i32(kept), _f32(weights_out), _i32(lengths_out),
-                                       _f32(weights_in), _i32(lengths), B, budget, recent), "kv_evict_paged")
+    f, i = src._float, src._int
+    _check(lib().kv_evict_paged_status(dst._ref, src._ref, _array(kept, i, (B, src.kv_heads, budget), "kept"),
+                                       _array(weights_out, f, (B, dst.kv_heads, dst.capacity), "weights_out"),
+                                       _array(lengths_out, i, (B,), "lengths_out"),
+                                       _array(weights_in, f, (B, src.kv_heads, src.capacity), "weights_in"),
+                                       _array(lengths, i, (B,), "lengths"), B, budget, recent), "kv_evict_paged")
 
 
 def argmax_forward(ids, logits, N, V):

@@ -232,8 +232,8 @@ struct Meeting {
   union {
     float o[W][GQ][ROW];
     struct {
-      float weight[GQ][kMaxRanges];
       f32x4 sum[W * kWave];
+      float m[W * kWave], l[W * kWave];
     } join;
   };
   float v[ROW];
@@ -339,8 +339,9 @@ __device__ __forceinline__ void finish(const AttendPaged& a, const Range& w, int
     } else {
       parts.store4((g * a.S + w.s) * a.part_stride + d, acc);
       if (d == 0) {
-        store_bypass(&a.part_ml[((bh0 + g) * a.S + w.s) * 2], top);
-        store_bypass(&a.part_ml[((bh0 + g) * a.S + w.s) * 2 + 1], sum);
+        const unsigned long long both = (unsigned long long)__builtin_bit_cast(unsigned, sum) << 32 | __builtin_bit_cast(unsigned, top);
+        __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.part_ml) + (bh0 + g) * a.S + w.s, both, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
       }
     }
   }
@@ -356,64 +357,79 @@ __device__ __forceinline__ void finish(const AttendPaged& a, const Range& w, int
   }
   __syncthreads();
   if (!meet.last) return;
-  // a wave per head: the ranges' weights, and the sum
-  const int lane = tid & 63;
-  for (int g = tid >> 6; g < w.heads; g += W) {
-    const float* ml = a.part_ml + (bh0 + g) * a.S * 2;
-    float m[kMaxRanges / 64], l[kMaxRanges / 64], top = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < kMaxRanges / 64; k++) {
-      const int s = lane + 64 * k;
-      m[k] = s < w.ranges ? load_bypass(ml + 2 * s) : -INFINITY;
-      l[k] = s < w.ranges ? load_bypass(ml + 2 * s + 1) : 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < kMaxRanges / 64; k++) top = fmaxf(top, m[k]);
-    top = wave_max(top);
-    const float base = above(top);
-    float sum = 0.f;
-#pragma unroll
-    for (int k = 0; k < kMaxRanges / 64; k++) {
-      const float x = __builtin_amdgcn_exp2f(m[k] - base);
-      meet.join.weight[g][lane + 64 * k] = x;
-      sum = fmaf(x, l[k], sum);
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) {
-      meet.l[0][g] = sum;
-      if (a.joined) {
-        a.joined[(bh0 + g) * 2] = base;
-        a.joined[(bh0 + g) * 2 + 1] = sum;
-      }
-    }
-  }
-  __syncthreads();
-  // as many threads per four channels as there are to spare, each with every so manieth range
+  // As many threads per four channels as there are to spare, each with every so manieth range and
+  // a softmax of its own over them; all loads of a thread are under way at once.
+  constexpr int MOST = 8;
   int per = 1;
   while (per < w.heads * HP4 && per < THREADS) per *= 2;
   const int slices = THREADS / per, slice = tid / per;
   for (int i0 = 0; i0 < w.heads * HP4; i0 += per) {
-    const int i = i0 + (tid & (per - 1));
-    const bool mine = i < w.heads * HP4;
-    const int g = mine ? i / HP4 : 0, d = mine ? (i - g * HP4) * 4 : 0;
+    const int i = min(i0 + (tid & (per - 1)), w.heads * HP4 - 1);
+    const int g = i / HP4, d = (i - g * HP4) * 4;
+    const unsigned long long* ml = reinterpret_cast<const unsigned long long*>(a.part_ml) + (bh0 + g) * a.S;
+    float m = -INFINITY, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (mine) {
-#pragma unroll 8
-      for (int s = slice; s < w.ranges; s += slices)
-        acc += meet.join.weight[g][s] * parts.load4((g * a.S + s) * a.part_stride + d);
+    for (int s0 = slice; s0 < w.ranges; s0 += MOST * slices) {
+      unsigned long long x[MOST];
+      f32x4 p[MOST];
+#pragma unroll
+      for (int u = 0; u < MOST; u++) {
+        const int s = s0 + u * slices;
+        x[u] = 0;
+        p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (s < w.ranges) {
+          x[u] = __hip_atomic_load(ml + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          p[u] = parts.load4((g * a.S + s) * a.part_stride + d);
+        }
+      }
+      float mu[MOST], top = m;
+#pragma unroll
+      for (int u = 0; u < MOST; u++) {
+        const unsigned bits = (unsigned)x[u];
+        mu[u] = s0 + u * slices < w.ranges ? __builtin_bit_cast(float, bits) : -INFINITY;
+        top = fmaxf(top, mu[u]);
+      }
+      const float base = above(top), fade = __builtin_amdgcn_exp2f(m - base);
+      m = top;
+      l *= fade;
+      acc *= fade;
+#pragma unroll
+      for (int u = 0; u < MOST; u++)
+        if (s0 + u * slices < w.ranges) {
+          const unsigned bits = (unsigned)(x[u] >> 32);
+          const float f = __builtin_amdgcn_exp2f(mu[u] - base);
+          l = fmaf(f, __builtin_bit_cast(float, bits), l);
+          acc += f * p[u];
+        }
     }
     if (slices > 1) {
       meet.join.sum[tid] = acc;
+      meet.join.m[tid] = m;
+      meet.join.l[tid] = l;
       __syncthreads();
-      if (slice == 0)
-        for (int k = 1; k < slices; k++) acc += meet.join.sum[tid + k * per];
+      if (slice == 0) {
+        float top = m;
+        for (int k = 1; k < slices; k++) top = fmaxf(top, meet.join.m[tid + k * per]);
+        const float base = above(top), fade = __builtin_amdgcn_exp2f(m - base);
+        m = top;
+        l *= fade;
+        acc *= fade;
+        for (int k = 1; k < slices; k++) {
+          const float f = __builtin_amdgcn_exp2f(meet.join.m[tid + k * per] - base);
+          l = fmaf(f, meet.join.l[tid + k * per], l);
+          acc += f * meet.join.sum[tid + k * per];
+        }
+      }
     }
-    if (mine && slice == 0) {
-      const float sum = meet.l[0][g];
+    if (slice == 0 && i0 + (tid & (per - 1)) < w.heads * HP4) {
       float* out = a.out + (bh0 + g) * HS + d;
 #pragma unroll
       for (int e = 0; e < 4; e++)
-        if (d + e < HS) out[e] = acc[e] / sum;
+        if (d + e < HS) out[e] = acc[e] / l;
+      if (d == 0 && a.joined) {
+        a.joined[(bh0 + g) * 2] = above(m);
+        a.joined[(bh0 + g) * 2 + 1] = l;
+      }
     }
   }
 }
@@ -445,6 +461,22 @@ __device__ __forceinline__ float rows_sum(float x, float y) {  // rows 0, 2: x's
   const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
   const unsigned lo = r[0], hi = r[1];
   return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+// The maximum across the lanes that are LPR and more apart, for every lane.
+template <int LPR>
+__device__ __forceinline__ float rows_max(float v) {
+  if constexpr (LPR <= 32) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned lo = h[0], hi = h[1];
+    v = fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+  }
+  if constexpr (LPR <= 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned lo = r[0], hi = r[1];
+    v = fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+  }
+  if constexpr (LPR <= 8) v = fmaxf(v, dpp<0x128>(v));  // row_ror:8
+  return v;
 }
 // The sums of four values over the four rows: row i of 16 lanes receives that of value quad_value(i).
 __device__ __forceinline__ float quads_sum(float x0, float x1, float x2, float x3) {
@@ -632,9 +664,7 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_kernel(const AttendP
   const bool all_ok = __ballot(!ok) == 0;
 #pragma unroll
   for (int g = 0; g < GQ; g++) {
-    float top = m[g];
-#pragma unroll
-    for (int off = LPR; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const float top = rows_max<LPR>(m[g]);
     const float fade = __builtin_amdgcn_exp2f(m[g] - above(top));
     float sum = l[g] * fade;
 #pragma unroll
@@ -793,8 +823,7 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const 
       }
     if constexpr (std::is_same<E, f16>::value) {
       // a power of two per head takes its largest entry to 2^13 .. 2^14
-      most = fmaxf(most, __shfl_xor(most, 16, 64));
-      most = fmaxf(most, __shfl_xor(most, 32, 64));
+      most = rows_max<16>(most);
       const int up = 14 - max(-100, min(100, __builtin_amdgcn_frexp_expf(most)));
       unscale = __builtin_amdgcn_ldexpf(1.f, -up);
 #pragma unroll
@@ -834,6 +863,7 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const 
       const E* src = (const E*)a.pg.keys + (size_t)__shfl(of, 16 * p + col, 64) * HS;
 #pragma unroll
       for (int j = 0; j < KS; j++) {
+        if (j > KS / 2 && 4 * PER * j >= HS) break;  // nothing but what is behind the row's end
         // behind the row's end: its last piece, against queries that are 0 there
         const int d = min(4 * PER * j + PER * quad, HS - PER);
         k[p][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + d));
@@ -881,15 +911,18 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const 
 #pragma unroll
       for (int i = NP - 1; i >= 0; i--)  // the smallest pieces first
 #pragma unroll
-        for (int j = 0; j < KS; j++)
+        for (int j = 0; j < KS; j++) {
+          if (j > KS / 2 && 4 * PER * j >= HS) break;
 #pragma unroll
           for (int p = 0; p < P16; p++) sc[p] = mfma32(k[p][j], q[i][j], sc[p], E{});
+        }
     } else {
 #pragma unroll
       for (int p = 0; p < P16; p++) {
         f32x4 s4[4] = {};  // four chains: a quarter of the roundings in each
 #pragma unroll
         for (int j = 0; j < KS; j++) {
+          if (j > KS / 2 && 4 * PER * j >= HS) break;
           const f32x4 kf = __builtin_bit_cast(f32x4, k[p][j]), qf = __builtin_bit_cast(f32x4, q[0][j]);
 #pragma unroll
           for (int e = 0; e < 4; e++) s4[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s4[e], 0, 0, 0);
@@ -949,8 +982,7 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const 
     float top = m;
 #pragma unroll
     for (int p = 0; p < P16; p++) top = fmaxf(top, fmaxf(fmaxf(sc[p][0], sc[p][1]), fmaxf(sc[p][2], sc[p][3])));
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = rows_max<16>(top);
     if (__ballot(top > m)) {
       const float fade = __builtin_amdgcn_exp2f(m - above(top));
       l *= fade;
@@ -1423,7 +1455,7 @@ static void launch_store(const Pages& pg, const float* inp, int stride, const in
 
 // Which kernel a problem takes, and how it is cut up.
 struct AttendPlan {
-  bool rows16, matrix;
+  bool rows16, matrix, deep;
   int gq, chunks, S, min_range, waves;
 };
 
@@ -1435,20 +1467,25 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
   p.gq = p.matrix ? kMatrixHeads : G >= 3 ? 4 : G;
   p.chunks = (G + p.gq - 1) / p.gq;
   const long long groups = (long long)B * c->kv_heads * p.chunks;
-  // few groups: large workgroups, whose waves need no memory to meet
-  const bool wide = groups <= 512;
-  p.waves = wide && p.rows16 && !(p.matrix && c->head_size > 128) ? 8 : 4;
-  // One workgroup per compute unit, or two where each has enough to do: the longest sequence's
-  // workgroups must not outlast the others'.  A range is worth a workgroup from 64 KB on.
+  // One workgroup of eight waves per compute unit, or, where that would leave many units idle and
+  // there is much to do, two that follow each other or share it.  From 257 to 512 workgroups the
+  // matrix kernel takes four waves, two workgroups of which fit a unit's registers (8 of 32 heads,
+  // fp32, 55 sequences: 25.2 -> 20.3 us).  Beyond, workgroups follow each other and need no
+  // splitting.  A range is worth a workgroup from 64 KB on.
   const long long row_bytes = 2LL * c->head_size * type_bytes(c->type), capacity = (long long)c->max_pages * c->page_size;
   p.min_range = (int)((65536 / row_bytes + 63) & ~63LL);
   if (p.min_range < 128) p.min_range = 128;
-  long long S = 512 / groups;
-  if (S < 1 || capacity * row_bytes / S < 512 * 1024) S = 256 / groups;
+  long long S = groups <= 256 ? 256 / groups : 0;
+  p.waves = 8;
+  if (S == 0 || (groups * S < 205 && capacity * row_bytes / S >= 768 * 1024)) S = 512 / groups;
+  if (groups > 512 || (p.matrix && groups > 256) || !p.rows16 || (p.matrix && c->head_size > 128)) p.waves = 4;
   const long long most = (capacity + p.min_range - 1) / p.min_range;
   if (S > most) S = most;
   if (groups * kCounterStride * 4 > GPT2HIP_PAGED_COUNTER_BYTES) S = 1;
   p.S = (int)(S < 1 ? 1 : S > kMaxRanges ? kMaxRanges : S);
+  // one workgroup per compute unit with much to do: twice the loads under way (16 sequences of 12
+  // heads, fp32, up to 1024 positions: 15.8 -> 15.0 us; short ranges would leave waves idle)
+  p.deep = groups * p.S <= 256 && capacity * row_bytes / p.S >= 256 * 1024;
   return p;
 }
 
@@ -1475,7 +1512,9 @@ static void launch_attend(const AttendPaged& a, const AttendPlan& p, unsigned bl
   else                                                                 \
     G2_KERNEL(4, attention_paged_matrix_kernel<E, CPL, P16, 4>);
 #define G2_ROWS(LPR)                                                   \
-  if (p.waves == 8 && p.gq == 1)                                       \
+  if (p.waves == 8 && p.gq == 1 && p.deep)                             \
+    G2_KERNEL(8, attention_paged_kernel<E, LPR, 1, 8, 8, false>);      \
+  else if (p.waves == 8 && p.gq == 1)                                  \
     G2_KERNEL(8, attention_paged_kernel<E, LPR, 1, 4, 8, false>);      \
   else if (p.waves == 8)                                               \
     G2_KERNEL(8, attention_paged_kernel<E, LPR, 2, 4, 8, false>);      \
