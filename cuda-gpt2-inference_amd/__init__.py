@@ -400,25 +400,28 @@ class PagedCache:
         self.page_size, self.capacity = size, size * table.shape[1]  # capacity: positions per sequence
         self._ref = ctypes.addressof(self._c)
         self._float, self._int = torch.float32, torch.int32
+        self._device, self._current_device = keys.get_device(), torch.cuda.current_device
+        if values.get_device() != self._device or table.get_device() != self._device:
+            raise ValueError("keys, values and table are on one GPU")
 
 
-def _array(t, dtype, shape, what) -> int:
-    """Device pointer of a contiguous CUDA tensor of that type and shape."""
+def _array(t, cache, dtype, shape, what) -> int:
+    """Device pointer of a contiguous tensor of that type and shape on the cache's GPU."""
     try:
-        if t.shape == shape and t.dtype is dtype and t.is_cuda and t.is_contiguous():
+        if t.shape == shape and t.dtype is dtype and t.get_device() == cache._device and t.is_contiguous():
             return t.data_ptr()
     except AttributeError:
         pass
-    if not hasattr(t, "is_cuda") or not t.is_cuda or t.dtype is not dtype:
-        raise TypeError(f"{what} is a {dtype} CUDA tensor, got {getattr(t, 'dtype', type(t))} on "
+    if not hasattr(t, "get_device") or t.get_device() != cache._device or t.dtype is not dtype:
+        raise TypeError(f"{what} is a {dtype} tensor on cuda:{cache._device}, got {getattr(t, 'dtype', type(t))} on "
                         f"{getattr(t, 'device', 'the host')}")
     raise ValueError(f"{what} is contiguous and {tuple(shape)}, got {tuple(t.shape)} with strides {t.stride()}")
 
 
-def _rows(inp, count, floats, dtype):
+def _rows(inp, cache, count, floats):
     """(pointer, stride in floats) of `count` rows of at least `floats` floats; a view of a wider array will do."""
-    if not hasattr(inp, "is_cuda") or not inp.is_cuda or inp.dtype is not dtype:
-        raise TypeError("expected a float32 CUDA tensor of rows")
+    if not hasattr(inp, "get_device") or inp.get_device() != cache._device or inp.dtype is not cache._float:
+        raise TypeError(f"expected float32 rows on cuda:{cache._device}")
     shape, strides = inp.shape, inp.stride()
     if len(shape) != 2 or shape[0] < count or shape[1] < floats or (shape[1] > 1 and strides[1] != 1):
         raise ValueError(f"expected {count} rows of {floats} consecutive floats, got {tuple(shape)} with strides {strides}")
@@ -426,14 +429,22 @@ def _rows(inp, count, floats, dtype):
     return inp.data_ptr(), strides[0] if count > 1 else max(strides[0], floats)
 
 
+def _on_its_gpu(cache, B) -> None:
+    """Launchers run on the current device: the cache has to be there, and to list B sequences."""
+    if cache._current_device() != cache._device:
+        raise ValueError(f"the cache is on cuda:{cache._device}, the current device is cuda:{cache._current_device()}")
+    if B > cache.sequences:
+        raise ValueError(f"the table lists {cache.sequences} sequences, asked for {B}")
+
+
 def kv_store_paged(cache, inp, starts, lengths, N, B, NH):
     """Store the keys and values of N packed rows (q | k | v; NH = 0: k | v) into the pages: rows
     starts[b] .. starts[b + 1] - 1 become positions lengths[b] and on of sequence b."""
-    if B > cache.sequences:
-        raise ValueError(f"the table lists {cache.sequences} sequences, asked for {B}")
-    rows, stride = _rows(inp, N, (NH + 2 * cache.kv_heads) * cache.head_size, cache._float)
-    _check(lib().kv_store_paged_status(cache._ref, rows, stride, _array(starts, cache._int, (B + 1,), "starts"),
-                                       _array(lengths, cache._int, (B,), "lengths"), N, B, NH), "kv_store_paged")
+    _on_its_gpu(cache, B)
+    rows, stride = _rows(inp, cache, N, (NH + 2 * cache.kv_heads) * cache.head_size)
+    i = cache._int
+    _check(lib().kv_store_paged_status(cache._ref, rows, stride, _array(starts, cache, i, (B + 1,), "starts"),
+                                       _array(lengths, cache, i, (B,), "lengths"), N, B, NH), "kv_store_paged")
 
 
 PAGED_COUNTER_BYTES = 65536  # GPT2HIP_PAGED_COUNTER_BYTES
@@ -455,34 +466,33 @@ def attention_decode_paged(out, cache, inp, lengths, B, NH, append=True, weights
     the new keys and values are stored as position lengths[b] first; otherwise inp holds queries
     that attend to the lengths[b] positions held.  weights_in, weights_out: accumulated attention
     weights (B, kv_heads, cache.capacity).  lengths[b] < 0: the row is left as it is."""
-    if B > cache.sequences:
-        raise ValueError(f"the table lists {cache.sequences} sequences, asked for {B}")
+    _on_its_gpu(cache, B)
     f, HS = cache._float, cache.head_size
-    rows, stride = _rows(inp, B, (NH + 2 * cache.kv_heads if append else NH) * HS, f)
+    rows, stride = _rows(inp, cache, B, (NH + 2 * cache.kv_heads if append else NH) * HS)
     win = wout = ws = None
     nbytes = 0
     if weights_in is not None:
-        win = _array(weights_in, f, (B, cache.kv_heads, cache.capacity), "weights_in")
+        win = _array(weights_in, cache, f, (B, cache.kv_heads, cache.capacity), "weights_in")
     if weights_out is not None:
-        wout = _array(weights_out, f, (B, cache.kv_heads, cache.capacity), "weights_out")
+        wout = _array(weights_out, cache, f, (B, cache.kv_heads, cache.capacity), "weights_out")
     if workspace is not None:
         ws, nbytes = _ptr(workspace), workspace.nbytes
-    _check(lib().attention_decode_paged_status(_array(out, f, (B, NH * HS), "out"), cache._ref, rows, stride,
-                                               _array(lengths, cache._int, (B,), "lengths"), win, wout, B, NH,
+    _check(lib().attention_decode_paged_status(_array(out, cache, f, (B, NH * HS), "out"), cache._ref, rows,
+                                               stride, _array(lengths, cache, cache._int, (B,), "lengths"), win, wout, B, NH,
                                                1 if append else 0, ws, nbytes), "attention_decode_paged")
 
 
 def kv_evict_paged(dst, src, kept, weights_out, lengths_out, weights_in, lengths, B, budget, recent):
     """Bring every sequence down to `budget` positions (the `recent` last ones and the heaviest of the
     others, each kv head for itself), copied from the pages of src into those of dst."""
-    if B > min(src.sequences, dst.sequences):
-        raise ValueError(f"the tables list {src.sequences} and {dst.sequences} sequences, asked for {B}")
+    _on_its_gpu(src, B)
+    _on_its_gpu(dst, B)
     f, i = src._float, src._int
-    _check(lib().kv_evict_paged_status(dst._ref, src._ref, _array(kept, i, (B, src.kv_heads, budget), "kept"),
-                                       _array(weights_out, f, (B, dst.kv_heads, dst.capacity), "weights_out"),
-                                       _array(lengths_out, i, (B,), "lengths_out"),
-                                       _array(weights_in, f, (B, src.kv_heads, src.capacity), "weights_in"),
-                                       _array(lengths, i, (B,), "lengths"), B, budget, recent), "kv_evict_paged")
+    _check(lib().kv_evict_paged_status(dst._ref, src._ref, _array(kept, src, i, (B, src.kv_heads, budget), "kept"),
+                                       _array(weights_out, src, f, (B, dst.kv_heads, dst.capacity), "weights_out"),
+                                       _array(lengths_out, src, i, (B,), "lengths_out"),
+                                       _array(weights_in, src, f, (B, src.kv_heads, src.capacity), "weights_in"),
+                                       _array(lengths, src, i, (B,), "lengths"), B, budget, recent), "kv_evict_paged")
 
 
 def argmax_forward(ids, logits, N, V):

@@ -102,6 +102,11 @@ class Case:
         return out.reshape(-1), tol.reshape(-1), p.sum(1), ptol
 
 
+def spread(count, top):
+    """count lengths of 0 .. top, short and long ones in turn, a few of them unused places."""
+    return [-1 if i % 23 == 22 else (i * 7919) % (top + 1) if i % 3 else (i * 31) % (top // 8 + 1) for i in range(count)]
+
+
 def same_bits(a, b):
     it = {4: torch.int32, 2: torch.int16}[a.element_size()]
     return torch.equal(a.cpu().view(it), b.cpu().view(it))
@@ -186,6 +191,24 @@ def test_attend_over_heads_and_types(kind, NH, KVH, HS):
     say(f"attend {kind} NH={NH} KVH={KVH} HS={HS}")
     lengths = [0, 1, 15, 16, 63, 131, 300]
     check_attend(Case(NH * 1000 + HS, kind, len(lengths), NH, KVH, HS, 16, lengths, 301))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("B,NH,KVH,HS,top,weights", [
+    (140, 4, 4, 64, 150, False),     # more than 512 (sequence, kv head) pairs: workgroups that follow each other
+    (140, 8, 4, 128, 150, True),     # the same, two query heads per kv head
+    (64, 4, 4, 64, 1100, True),      # one workgroup per compute unit with much to do
+    (64, 4, 4, 128, 600, False), (64, 4, 4, 256, 300, False), (64, 4, 4, 32, 2100, False),
+    (90, 12, 3, 64, 200, True),      # matrix kernel: 270 pairs
+    (90, 15, 3, 128, 100, False), (90, 12, 3, 256, 60, False),
+    (170, 16, 4, 64, 60, False),     # and more than 512
+    (2, 20, 1, 96, 9000, True),      # few pairs, long, more heads than a workgroup takes
+    (3, 1, 1, 64, 20000, True),
+])
+def test_attend_every_form_of_the_kernels(kind, B, NH, KVH, HS, top, weights):
+    """Sizes on both sides of every line that the plan of a call draws."""
+    say(f"attend {kind} B={B} NH={NH} KVH={KVH} HS={HS} top={top}")
+    check_attend(Case(B + HS, kind, B, NH, KVH, HS, 16, spread(B, top), top + 1), weights=weights)
 
 
 @pytest.mark.parametrize("page", [1, 3, 16, 24, 128, 1000])
@@ -706,3 +729,31 @@ def test_decoding_equals_the_causal_attention_row_by_row():
     for t in range(T):
         g2.attention_decode_paged(out, cache, qkv[:, t], torch.full((B,), t, dtype=torch.int32, device="cuda"), B, NH)
         assert torch.allclose(out, whole[:, t], rtol=2e-4, atol=2e-5), t
+
+
+def test_a_cache_on_another_gpu_is_refused():
+    c = Case(30, "f32", 1, 1, 1, 64, 16, [5], 16)
+    cache = c.gpu()
+    out = torch.zeros((1, 64), device="cuda")
+    cache._device += 1  # as if its tensors lay there
+    with pytest.raises(ValueError, match="current device"):
+        g2.attention_decode_paged(out, cache, c.inp.cuda(), c.dl, 1, 1)
+    with pytest.raises(ValueError, match="current device"):
+        g2.kv_store_paged(cache, c.inp.cuda(), torch.zeros(2, dtype=torch.int32, device="cuda"), c.dl, 1, 1, 1)
+
+
+def test_python_refusals():
+    c = Case(31, "f32", 2, 2, 1, 64, 16, [5, 6], 32)
+    cache = c.gpu()
+    inp, out = c.inp.cuda(), torch.zeros((2, 128), device="cuda")
+    ok = dict(out=out, cache=cache, inp=inp, lengths=c.dl, B=2, NH=2)
+    for other, error in ((dict(out=out.double()), TypeError), (dict(out=out.cpu()), TypeError), (dict(out=out[:, :64]), ValueError),
+                         (dict(out=out.t().contiguous().t()), ValueError), (dict(lengths=c.dl.long()), TypeError),
+                         (dict(lengths=c.dl[:1]), ValueError), (dict(inp=inp[:, :-1]), ValueError), (dict(inp=inp[:1]), ValueError),
+                         (dict(inp=inp.t()), ValueError), (dict(inp=inp.cpu()), TypeError), (dict(B=3), ValueError),
+                         (dict(weights_in=torch.zeros((2, 1, 32), device="cuda")), g2.GPT2HipError),
+                         (dict(weights_in=torch.zeros((2, 1, 31), device="cuda")), ValueError)):
+        with pytest.raises(error):
+            g2.attention_decode_paged(**{**ok, **other})
+    g2.attention_decode_paged(**ok)
+    torch.cuda.synchronize()
