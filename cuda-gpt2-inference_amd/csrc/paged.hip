@@ -1156,43 +1156,34 @@ __device__ __forceinline__ int waves_sum(int v) {
 
 constexpr int kFew = 4096;  // ranks that are worth a list of their own
 
-// One workgroup per (sequence, kv head) chooses the positions that stay: the `recent` last ones
-// and, of the others, the budget - recent of largest weight.  The smallest rank that stays is
-// found two bits at a time by counting how many ranks go each of the four ways: sums of integers,
-// the same on every run.  Once few ranks are left that could be it, they are listed in
-// LDS and the rest is not looked at again until the end; the search ends early where a candidate
-// is reached by exactly as many ranks as are wanted.  A wave owns consecutive positions, so that the
-// places in the output follow from counts alone.  R ranks per thread are kept in registers;
-// R = 0: any length, read again for every count.
-template <int WAVES, int R>
-__global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
-    int* __restrict__ kept, int* __restrict__ lengths_out, const float* __restrict__ weights,
-    const int* __restrict__ lengths, int KVH, int capacity, int budget, int recent) {
+struct Evict {
+  Pages dst, src;
+  int* kept;
+  float* weights_out;
+  int* lengths_out;
+  const float* weights_in;
+  const int* lengths;
+  int B, budget, recent;
+  int row_bytes, rows, groups;  // rows that a wave copies, waves (or, with the choice, workgroups) per (sequence, kv head)
+};
+
+// Which of the `older` first positions stay: the `want` (0 < want < older) of largest weight w,
+// for each of which put(place, position) is called.  A workgroup of WAVES waves, all of it.
+// The smallest rank that stays is found two bits at a time by counting how many ranks go each of
+// the four ways: sums of integers, the same on every run.  Once few ranks are left that could be
+// it, they are listed in LDS and the rest is not looked at again until the end; the search ends
+// early where a candidate is reached by exactly as many ranks as are wanted.  A wave owns
+// consecutive positions, so that the places in the output follow from counts alone.  R ranks per
+// thread are kept in registers; R = 0: any length, read again for every count.
+template <int WAVES, int R, class Put>
+__device__ __forceinline__ void pick(const float* __restrict__ w, int older, int want, int tid, Put put) {
   constexpr int THREADS = WAVES * kWave;
   constexpr bool LISTS = R == 0 || R * THREADS > 2 * kFew;
   constexpr int FEW = LISTS ? kFew / THREADS : 1;
   __shared__ unsigned list[LISTS ? kFew : 1];
   __shared__ int counts[2][WAVES][3], waves[2][WAVES], listed;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const size_t bh = blockIdx.x;
-  const int b = (int)(bh / KVH);
+  const int lane = tid & 63, wave = tid >> 6;
   if (tid == 0) listed = 0;
-  const int n = lengths[b];
-  if (n < 0) return;
-  const bool too_long = n > capacity;
-  const int stay = too_long ? 0 : min(n, budget);
-  if (bh % KVH == 0 && tid == 0) lengths_out[b] = too_long ? -1 : stay;
-  int* out = kept + bh * budget;
-  for (int j = stay + tid; j < budget; j += THREADS) out[j] = -1;
-  if (stay == n || too_long) {  // nothing has to go
-    for (int j = tid; j < stay; j += THREADS) out[j] = j;
-    return;
-  }
-  const int older = n - recent, want = budget - recent;  // want < older
-  for (int j = tid; j < recent; j += THREADS) out[want + j] = older + j;
-  if (want == 0) return;
-
-  const float* w = weights + bh * capacity;
   const int span = R ? 64 * R : ((older + WAVES - 1) / WAVES + 63) & ~63;
   const int first = wave * span, groups = R ? R : span / 64;
   unsigned rank[R ? R : 1];
@@ -1324,7 +1315,7 @@ __global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
     each([&](int r, unsigned x) {
       const unsigned long long g = __ballot(x >= low);
       const int at = lanes_before(g, gt_before);
-      if (x >= low && at < want) out[at] = first + r * 64 + lane;
+      if (x >= low && at < want) put(at, first + r * 64 + lane);
       gt_before += __popcll(g);
     });
     return;
@@ -1333,53 +1324,36 @@ __global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(
   each([&](int r, unsigned x) {
     const unsigned long long g = __ballot(x > low), e = __ballot(x == low);
     const int eq_at = lanes_before(e, eq_before), at = lanes_before(g, gt_before) + min(eq_at, room);
-    if ((x > low || (x == low && eq_at < room)) && at < want) out[at] = first + r * 64 + lane;
+    if ((x > low || (x == low && eq_at < room)) && at < want) put(at, first + r * 64 + lane);
     gt_before += __popcll(g);
     eq_before += __popcll(e);
   });
 }
 
-// Copies what stays into the pages of the other table.  A wave moves the keys and values of
-// kCopyLoads times as many rows of one (sequence, kv head) as one load of it holds, all loads
-// ahead of the stores, and their weights.  UNIT: bytes per lane and load, 16 or the size of an
-// element.
+// Copies the keys and values of `rows` rows of one (sequence, kv head), kCopyLoads times as many
+// as one load of the wave holds, all loads ahead of the stores, and their weights.  Lane r < rows
+// says that row j comes from position i.  UNIT: bytes per lane and load, 16 or the size of an
+// element; STREAM: stores past the caches (rows of whole cache lines).
 constexpr int kCopyLoads = 4;
 static int copy_rows(int row_bytes, int unit) {  // rows per wave
   const int units = row_bytes / unit, per = units < 64 ? 64 / units : 1;
   return per * kCopyLoads < 64 ? per * kCopyLoads : 64;
 }
 template <int UNIT, bool STREAM>
-__global__ __launch_bounds__(256) void kv_evict_copy_kernel(Pages dst, Pages src, const int* __restrict__ kept,
-                                                            float* __restrict__ weights_out,
-                                                            const float* __restrict__ weights_in,
-                                                            const int* __restrict__ lengths, int B, int budget,
-                                                            int row_bytes, int rows, int groups) {
-  const int lane = threadIdx.x & 63;
-  const size_t id = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int KVH = src.kv_heads;
-  const size_t bh = id / groups;
-  const int b = (int)(bh / KVH), h = (int)(bh % KVH);
-  if (b >= B) return;
-  const int j0 = (int)(id % groups) * rows, j = j0 + lane;
-  const int n = lengths[b];
-  if (n < 0 || n > src.capacity) return;
-  const int stay = min(n, budget);
-  if (j0 >= stay) return;
+__device__ __forceinline__ void copy_kept(const Evict& e, size_t bh, int b, int h, int lane, bool ok, int i, int j) {
   unsigned from = 0, to = 0;
-  bool ok = lane < rows && j < stay;
   if (ok) {
-    const int i = min(max(kept[bh * budget + j], 0), n - 1);
-    const float w = weights_in[bh * src.capacity + i];
-    from = src.row(b, h, i, ok);
-    to = dst.row(b, h, j, ok);
-    weights_out[bh * dst.capacity + j] = ok ? w : __builtin_nanf("");
+    const float w = e.weights_in[bh * e.src.capacity + i];
+    from = e.src.row(b, h, i, ok);
+    to = e.dst.row(b, h, j, ok);
+    e.weights_out[bh * e.dst.capacity + j] = ok ? w : __builtin_nanf("");
   }
   const unsigned long long live = __ballot(ok);
-  const int units = row_bytes / UNIT, per = units < 64 ? 64 / units : 1;  // units per row, rows per load
+  const int units = e.row_bytes / UNIT, per = units < 64 ? 64 / units : 1;  // units per row, rows per load
   const int mine = lane / units;
   typedef typename std::conditional<UNIT == 16, u32x4, typename std::conditional<UNIT == 4, unsigned, unsigned short>::type>::type Word;
-  const Word *ks = (const Word*)src.keys, *vs = (const Word*)src.values;
-  Word *kd = (Word*)dst.keys, *vd = (Word*)dst.values;
+  const Word *ks = (const Word*)e.src.keys, *vs = (const Word*)e.src.values;
+  Word *kd = (Word*)e.dst.keys, *vd = (Word*)e.dst.values;
   const int c0 = lane - mine * units;  // a row of more than 64 units takes more than one round, all lanes in each
   for (int round = 0; round < units; round += 64) {
     const int c = min(c0 + round, units - 1);
@@ -1394,7 +1368,7 @@ __global__ __launch_bounds__(256) void kv_evict_copy_kernel(Pages dst, Pages src
     for (int u = 0; u < kCopyLoads; u++) {
       const int r = u * per + mine;
       const size_t x = (size_t)__shfl(to, r & 63, 64) * units + c;
-      if (mine < per && r < rows && c0 + round < units && ((live >> (r & 63)) & 1ull)) {
+      if (mine < per && r < e.rows && c0 + round < units && ((live >> (r & 63)) & 1ull)) {
         if constexpr (STREAM) {
           __builtin_nontemporal_store(k[u], kd + x);
           __builtin_nontemporal_store(v[u], vd + x);
@@ -1405,6 +1379,65 @@ __global__ __launch_bounds__(256) void kv_evict_copy_kernel(Pages dst, Pages src
       }
     }
   }
+}
+
+// One workgroup per (sequence, kv head) chooses the positions that stay: the `recent` last ones
+// and, of the others, the budget - recent of largest weight.
+// COPY (caches of up to some thousand positions, where a second launch would cost as much as the
+// choice): several workgroups per (sequence, kv head), each of which makes the whole choice and
+// copies its share of the rows.
+template <int WAVES, int R, bool COPY, int UNIT, bool STREAM>
+__global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(const Evict e) {
+  constexpr int THREADS = WAVES * kWave;
+  __shared__ int here[COPY ? WAVES * 64 : 1];  // this workgroup's share of the positions
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int KVH = e.src.kv_heads;
+  const size_t bh = COPY ? blockIdx.x / (unsigned)e.groups : blockIdx.x;
+  const int b = (int)(bh / KVH), h = (int)(bh % KVH);
+  const int share = COPY ? WAVES * e.rows : e.budget;
+  const int j0 = COPY ? (int)(blockIdx.x % (unsigned)e.groups) * share : 0, j1 = min(j0 + share, e.budget);
+  const int n = e.lengths[b];
+  if (n < 0) return;
+  const bool too_long = n > e.src.capacity;
+  const int stay = too_long ? 0 : min(n, e.budget);
+  if (h == 0 && j0 == 0 && tid == 0) e.lengths_out[b] = too_long ? -1 : stay;
+  int* out = e.kept + bh * e.budget;
+  for (int j = max(stay, j0) + tid; j < j1; j += THREADS) out[j] = -1;
+  if (j0 >= stay) return;
+  auto put = [&](int j, int i) {
+    if constexpr (COPY) {
+      if (j < j0 || j >= j1) return;
+      here[j - j0] = i;
+    }
+    out[j] = i;
+  };
+  if (stay == n) {  // nothing has to go
+    for (int j = j0 + tid; j < min(j1, stay); j += THREADS) put(j, j);
+  } else {
+    const int older = n - e.recent, want = e.budget - e.recent;  // want < older
+    for (int j = max(want, j0) + tid; j < j1; j += THREADS) put(j, older + j - want);
+    if (want > j0) pick<WAVES, R>(e.weights_in + bh * e.src.capacity, older, want, tid, put);
+  }
+  if constexpr (COPY) {
+    __syncthreads();
+    const int r = wave * e.rows + lane, j = j0 + r;
+    const bool ok = lane < e.rows && j < min(j1, stay);
+    copy_kept<UNIT, STREAM>(e, bh, b, h, lane, ok, ok ? min(max(here[r], 0), n - 1) : 0, j);
+  }
+}
+
+template <int UNIT, bool STREAM>
+__global__ __launch_bounds__(256) void kv_evict_copy_kernel(const Evict e) {
+  const int lane = threadIdx.x & 63;
+  const size_t id = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const size_t bh = id / e.groups;
+  const int b = (int)(bh / e.src.kv_heads), h = (int)(bh % e.src.kv_heads);
+  if (b >= e.B) return;
+  const int j0 = (int)(id % e.groups) * e.rows, j = j0 + lane;
+  const int n = e.lengths[b];
+  if (n < 0 || n > e.src.capacity || j0 >= min(n, e.budget)) return;
+  const bool ok = lane < e.rows && j < min(n, e.budget);
+  copy_kept<UNIT, STREAM>(e, bh, b, h, lane, ok, ok ? min(max(e.kept[bh * e.budget + j], 0), n - 1) : 0, j);
 }
 
 // ---- launchers ------------------------------------------------------------------------------
@@ -1674,20 +1707,51 @@ int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, 
   if (weights_out == weights_in || lengths_out == lengths)
     return fail(GPT2HIP_EINVAL, "kv_evict_paged: weights_out and lengths_out must not be the inputs");
   const int KVH = from.kv_heads;
-  const int row_bytes = (int)(from.head_size * type_bytes(src->type));
+  Evict e{to, from, kept, weights_out, lengths_out, weights_in, lengths, B, budget, recent, 0, 0, 0};
+  e.row_bytes = (int)(from.head_size * type_bytes(src->type));
   const int unit = rows_by_16(src) && rows_by_16(dst) ? 16 : (int)type_bytes(src->type);
-  const int rows = copy_rows(row_bytes, unit), groups = (budget + rows - 1) / rows;
-  const long long pairs = (long long)B * KVH, blocks = (pairs * groups + 3) / 4;
-  if (pairs > 0x7fffffffLL || blocks > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "kv_evict_paged: grid too large");
+  e.rows = copy_rows(e.row_bytes, unit);
   const int most = from.capacity - recent;  // weights that can take part
-#define G2_PICK(WAVES, R)                                                                                   \
-  hipLaunchKernelGGL((kv_evict_pick_kernel<WAVES, R>), dim3((unsigned)pairs), dim3(WAVES * kWave), 0, stream(), kept, \
-                     lengths_out, weights_in, lengths, KVH, from.capacity, budget, recent)
-  if (most <= 256)
-    G2_PICK(4, 1);
-  else if (most <= 1024)
-    G2_PICK(4, 4);
-  else if (most <= 4 * 1024)
+  // Choice and copy in one launch, the choice made again by every workgroup: up to 4096 weights,
+  // and not where many workgroups would copy nearly everything (48 pairs, 2000 -> 1000 positions:
+  // 17.2 -> 14.0 us; 768 pairs, 185 -> 168; but 768 pairs, 4000 -> 3600: 318 -> 375).
+  const long long pairs = (long long)B * KVH, groups4 = (budget + 4 * e.rows - 1) / (4 * e.rows);
+  const bool together = most <= 4096 && (4LL * budget <= 3LL * from.capacity || pairs * groups4 <= 1024);
+  e.groups = together ? (int)groups4 : (budget + e.rows - 1) / e.rows;
+  const long long copies = together ? pairs * e.groups : (pairs * e.groups + 3) / 4;
+  if (pairs > 0x7fffffffLL || copies > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "kv_evict_paged: grid too large");
+#define G2_UNITS(KERNEL)                                                                           \
+  if (unit == 16 && e.row_bytes % 128 == 0) /* whole cache lines */                                \
+    KERNEL(16, true);                                                                              \
+  else if (unit == 16)                                                                             \
+    KERNEL(16, false);                                                                             \
+  else if (unit == 4)                                                                              \
+    KERNEL(4, false);                                                                              \
+  else                                                                                             \
+    KERNEL(2, false);
+#define G2_BOTH_1(UNIT, STREAM) \
+  hipLaunchKernelGGL((kv_evict_pick_kernel<4, 1, true, UNIT, STREAM>), dim3((unsigned)copies), dim3(256), 0, stream(), e)
+#define G2_BOTH_4(UNIT, STREAM) \
+  hipLaunchKernelGGL((kv_evict_pick_kernel<4, 4, true, UNIT, STREAM>), dim3((unsigned)copies), dim3(256), 0, stream(), e)
+#define G2_BOTH_16(UNIT, STREAM) \
+  hipLaunchKernelGGL((kv_evict_pick_kernel<4, 16, true, UNIT, STREAM>), dim3((unsigned)copies), dim3(256), 0, stream(), e)
+#define G2_PICK(WAVES, R)                                                                                               \
+  hipLaunchKernelGGL((kv_evict_pick_kernel<WAVES, R, false, 16, false>), dim3((unsigned)pairs), dim3(WAVES * kWave), 0, \
+                     stream(), e)
+#define G2_COPY(UNIT, STREAM) \
+  hipLaunchKernelGGL((kv_evict_copy_kernel<UNIT, STREAM>), dim3((unsigned)copies), dim3(256), 0, stream(), e)
+  if (together) {
+    if (most <= 256) {
+      G2_UNITS(G2_BOTH_1)
+    } else if (most <= 1024) {
+      G2_UNITS(G2_BOTH_4)
+    } else {
+      G2_UNITS(G2_BOTH_16)
+    }
+    G2_LAUNCH_CHECK("kv_evict_paged");
+    return GPT2HIP_OK;
+  }
+  if (most <= 4 * 1024)
     G2_PICK(16, 4);
   else if (most <= 16 * 1024)
     G2_PICK(16, 16);
@@ -1695,21 +1759,14 @@ int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, 
     G2_PICK(16, 32);
   else
     G2_PICK(16, 0);
-#undef G2_PICK
   G2_LAUNCH_CHECK("kv_evict_paged (choice)");
-  const dim3 grid((unsigned)blocks), block(256);
-#define G2_COPY(UNIT, STREAM)                                                                                             \
-  hipLaunchKernelGGL((kv_evict_copy_kernel<UNIT, STREAM>), grid, block, 0, stream(), to, from, kept, weights_out, weights_in, \
-                     lengths, B, budget, row_bytes, rows, groups)
-  if (unit == 16 && row_bytes % 128 == 0)  // whole cache lines
-    G2_COPY(16, true);
-  else if (unit == 16)
-    G2_COPY(16, false);
-  else if (unit == 4)
-    G2_COPY(4, false);
-  else
-    G2_COPY(2, false);
+  G2_UNITS(G2_COPY)
 #undef G2_COPY
+#undef G2_PICK
+#undef G2_BOTH_16
+#undef G2_BOTH_4
+#undef G2_BOTH_1
+#undef G2_UNITS
   G2_LAUNCH_CHECK("kv_evict_paged (copy)");
   return GPT2HIP_OK;
 }

@@ -396,6 +396,95 @@ def test_attend_is_repeatable_and_replays_in_a_graph():
         assert torch.equal(out, want[0]) and torch.equal(wo, want[1]), lengths
 
 
+def test_calls_of_different_sizes_share_a_workspace_one_after_the_other():
+    cases = [Case(40 + i, kind, B, NH, KVH, 64, 16, lengths, max(lengths) + 1)
+             for i, (kind, B, NH, KVH, lengths) in enumerate([
+                 ("f32", 2, 3, 3, [2000, 900]), ("bf16", 1, 8, 1, [3000]), ("f16", 7, 4, 2, [10, 500, 3, 900, 64, 0, 77]),
+                 ("f32", 1, 1, 1, [5000])])]
+    caches = [c.gpu() for c in cases]
+    need = max(g2.attention_decode_paged_workspace(k, c.B, c.NH, weights=True).numel() for k, c in zip(caches, cases))
+    shared = torch.zeros(need, dtype=torch.uint8, device="cuda")
+
+    def run(i, ws):
+        c = cases[i]
+        out = torch.zeros((c.B, c.NH * 64), device="cuda")
+        w = torch.zeros((c.B, c.KVH, c.cap), device="cuda")
+        own = ws if ws is not None else g2.attention_decode_paged_workspace(caches[i], c.B, c.NH, weights=True)
+        g2.attention_decode_paged(out, caches[i], c.inp.cuda(), c.dl, c.B, c.NH, weights_in=w, weights_out=w, workspace=own)
+        return out, w
+
+    alone = [run(i, None) for i in range(4)]
+    for i in (0, 1, 2, 3, 3, 1, 0, 2, 1, 2, 0, 3):
+        # a larger workspace than a call asks for changes nothing
+        got = run(i, shared)
+        assert torch.equal(got[0], alone[i][0]) and torch.equal(got[1], alone[i][1]), i
+    assert (shared[: g2.PAGED_COUNTER_BYTES] == 0).all()
+
+
+def test_two_streams_with_a_workspace_each():
+    """Calls that overlap on the GPU: the same bits as one after the other."""
+    cases = [Case(50, "f32", 2, 3, 3, 64, 16, [3000, 900], 3001), Case(51, "bf16", 2, 16, 2, 128, 16, [2500, 3000], 3001)]
+    caches = [c.gpu() for c in cases]
+    inps = [c.inp.cuda() for c in cases]
+    spaces = [g2.attention_decode_paged_workspace(k, 2, c.NH) for k, c in zip(caches, cases)]
+    outs = [torch.zeros((8, 2, c.NH * c.HS), device="cuda") for c in cases]
+    want = []
+    for i in range(2):
+        g2.attention_decode_paged(outs[i][0], caches[i], inps[i], cases[i].dl, 2, cases[i].NH, workspace=spaces[i])
+        want.append(outs[i][0].clone())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    try:
+        for k in range(8):
+            for i in range(2):
+                g2.set_stream(streams[i])
+                g2.attention_decode_paged(outs[i][k], caches[i], inps[i], cases[i].dl, 2, cases[i].NH, workspace=spaces[i])
+    finally:
+        g2.set_stream(None)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(outs[i][k], want[i]) for k in range(8))
+
+
+def test_store_and_evict_replay_in_a_graph():
+    g = torch.Generator().manual_seed(60)
+    B, KVH, HS, page, P = 3, 2, 64, 16, 6
+    pages = torch.randperm(2 * B * P, generator=g).to(torch.int32).view(2, B, P).cuda()
+    keys, values = (torch.randn((2 * B * P, KVH, page, HS), generator=g).cuda() for _ in range(2))
+    src, dst = g2.PagedCache(keys, values, pages[0]), g2.PagedCache(keys, values, pages[1])
+    rows = torch.randn((60, 2 * KVH * HS), generator=g).cuda()
+    starts, held = torch.tensor([0, 20, 50, 60], dtype=torch.int32).cuda(), torch.zeros(3, dtype=torch.int32).cuda()
+    lengths, weights = torch.zeros(3, dtype=torch.int32).cuda(), torch.rand((B, KVH, P * page), generator=g).cuda()
+    kept = torch.zeros((B, KVH, 40), dtype=torch.int32).cuda()
+    wo, lo = torch.zeros_like(weights), torch.zeros_like(lengths)
+
+    def call():
+        g2.kv_store_paged(src, rows, starts, held, 60, B, 0)
+        g2.kv_evict_paged(dst, src, kept, wo, lo, weights, lengths, B, 40, 5)
+
+    call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            g2.set_stream(side)
+            call()
+    finally:
+        g2.set_stream(None)
+    for at, n in (([0, 0, 0], [20, 30, 10]), ([30, 5, 80], [50, 35, 90]), ([0, -1, 7], [20, -1, 17])):
+        state = []
+        for replay in (False, True):
+            keys.copy_(torch.arange(keys.numel(), device="cuda").view_as(keys) % 997), values.copy_(-keys)
+            rows.mul_(1.0), kept.fill_(-9), wo.fill_(-5), lo.fill_(-9)
+            held.copy_(torch.tensor(at, dtype=torch.int32)), lengths.copy_(torch.tensor(n, dtype=torch.int32))
+            torch.cuda.synchronize()
+            graph.replay() if replay else call()
+            torch.cuda.synchronize()
+            state.append([t.clone() for t in (keys, values, kept, wo, lo)])
+        assert all(torch.equal(x, y) for x, y in zip(*state)), n
+
+
 def test_attend_pool_beyond_32_bit_offsets():
     """Pages whose first element lies behind 2^32 elements: 2^18 pages of (2, 64, 256) bf16 and more."""
     NH, KVH, HS, page = 4, 2, 256, 64
@@ -622,6 +711,11 @@ def negative(B, KVH, cap, g):
 @pytest.mark.parametrize("n,budget", [(300, 100), (9001, 8000), (20000, 19000), (20000, 40)])
 def test_evict_negative_weights(n, budget):
     check_evict(8, "f32", [n, n - 7], budget, 10, KVH=1, HS=8, page=64, weights=negative)
+
+
+def test_evict_many_that_stay_nearly_whole():
+    """More than a thousand (sequence, kv head) pairs, most positions stay: choice and copy apart."""
+    check_evict(10, "bf16", [48 - i % 9 for i in range(520)], 40, 3, KVH=2, HS=8, page=8)
 
 
 def test_evict_one_value_apart():
