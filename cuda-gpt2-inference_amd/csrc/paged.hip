@@ -59,13 +59,13 @@ __device__ __forceinline__ void widen16(float (&to)[8], u32x4 raw, bf16) {
 }
 
 // ---- position -> row of the pages -----------------------------------------------------------
-// Division by the page size as one high product and a shift, exact for every 31-bit position:
-// with shift = ceil(log2 d) and magic = ceil(2^(31 + shift) / d), magic fits 32 bits and
-// floor(n * magic / 2^(31 + shift)) = floor(n / d) for n < 2^31, because magic * d exceeds
-// 2^(31 + shift) by less than d <= 2^shift.
+// Division by the page size as one product and a shift, exact for every 31-bit position:
+// with log = ceil(log2 d) and magic = ceil(2^(31 + log) / d), magic fits 32 bits and
+// floor(n * magic / 2^(31 + log)) = floor(n / d) for n < 2^31, because magic * d exceeds
+// 2^(31 + log) by less than d <= 2^log.
 struct PageDivide {
   unsigned magic;
-  int shift;  // after the high half of the 64-bit product: 31 + log - 32
+  int shift;  // 31 + log
   unsigned size;
   explicit PageDivide(int d = 1) : size((unsigned)d) {
     int log = 0;
@@ -1500,25 +1500,31 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
   p.gq = p.matrix ? kMatrixHeads : G >= 3 ? 4 : G;
   p.chunks = (G + p.gq - 1) / p.gq;
   const long long groups = (long long)B * c->kv_heads * p.chunks;
+  const long long capacity = (long long)c->max_pages * c->page_size, row_bytes = 2LL * c->head_size * type_bytes(c->type);
+  const long long each = capacity * row_bytes;  // of keys and values, per group
   // One workgroup of eight waves per compute unit, or, where that would leave many units idle and
-  // there is much to do, two that follow each other or share it.  From 257 to 512 workgroups the
-  // matrix kernel takes four waves, two workgroups of which fit a unit's registers (8 of 32 heads,
-  // fp32, 55 sequences: 25.2 -> 20.3 us).  Beyond, workgroups follow each other and need no
-  // splitting.  A range is worth a workgroup from 64 KB on.
-  const long long row_bytes = 2LL * c->head_size * type_bytes(c->type), capacity = (long long)c->max_pages * c->page_size;
+  // there is much to do, two that follow each other or share it: a split costs 3-4 us (parts to
+  // memory, the counter, parts back), so that short caches are left whole.  A range is worth a
+  // workgroup from 64 KB on.  Beyond 512 groups workgroups follow each other and nothing is split.
   p.min_range = (int)((65536 / row_bytes + 63) & ~63LL);
   if (p.min_range < 128) p.min_range = 128;
   long long S = groups <= 256 ? 256 / groups : 0;
-  p.waves = 8;
-  if (S == 0 || (groups * S < 205 && capacity * row_bytes / S >= 768 * 1024)) S = 512 / groups;
-  if (groups > 512 || (p.matrix && groups > 256) || !p.rows16 || (p.matrix && c->head_size > 128)) p.waves = 4;
-  const long long most = (capacity + p.min_range - 1) / p.min_range;
-  if (S > most) S = most;
+  if (S == 0 || (groups * S < 205 && each / S >= 768 * 1024)) S = 512 / groups;
+  if (S > capacity / p.min_range) S = capacity / p.min_range;
   if (groups * kCounterStride * 4 > GPT2HIP_PAGED_COUNTER_BYTES) S = 1;
+  // Four waves instead of eight for many short caches (64 sequences of 12 heads, bf16, up to 100
+  // positions: 7.0 against 9.3 us; 64 of 16 heads of 128 channels, up to 2000: 135 against 130)
+  // and where eight would take all of a unit's registers: the matrix kernel from 257 groups on
+  // (8 of 32 heads, fp32, 55 sequences: 20.3 against 25.2 us) and for head sizes above 128 -- or
+  // where four have one tile each and no more (30 sequences of 8 of 32 heads, fp16, up to 60: 6.9
+  // against 7.4 us).
+  p.waves = 8;
+  if (!p.rows16 || (groups > 512 && each < 768 * 1024)) p.waves = 4;
+  if (p.matrix && (groups > 256 || (capacity <= 128 && type_bytes(c->type) == 2) || c->head_size > 128)) p.waves = 4;
   p.S = (int)(S < 1 ? 1 : S > kMaxRanges ? kMaxRanges : S);
   // one workgroup per compute unit with much to do: twice the loads under way (16 sequences of 12
   // heads, fp32, up to 1024 positions: 15.8 -> 15.0 us; short ranges would leave waves idle)
-  p.deep = groups * p.S <= 256 && capacity * row_bytes / p.S >= 256 * 1024;
+  p.deep = groups * p.S <= 256 && each / p.S >= 256 * 1024;
   return p;
 }
 

@@ -223,9 +223,9 @@ int matmul_forward_argmax_noalloc_status(int* ids, const float* inp, const float
  * Any head_size up to 256, any page_size, any kv_heads that divides NH.  A row takes fast paths
  * where it is a multiple of 16 bytes and keys and values are 16-byte aligned.
  * lengths (B, int32, on the device) says how many positions each sequence holds; a negative one
- * marks an unused place in the batch: nothing of it is read or written, and its rows of every
+ * marks an unused place in the batch: no page of it is read or written, and its rows of every
  * output stay as they were.  Table entries outside [0, num_pages) are never followed: see each
- * call.  Entries behind a sequence's last position are not read.  Nothing is allocated, nothing
+ * call; nor are entries behind a sequence's last position, which may hold anything.  Nothing is allocated, nothing
  * synchronises, nothing is kept between calls: the calls can be captured in a graph. */
 enum { GPT2HIP_F32 = 0, GPT2HIP_F16 = 1, GPT2HIP_BF16 = 2 };
 typedef struct {
@@ -255,14 +255,15 @@ int kv_store_paged_status(const GPT2PagedCache* cache, const float* inp, int inp
  * stored as position lengths[b] (the caller advances lengths) and the query attends to positions
  * 0 .. lengths[b].  append == 0: only the queries of inp are read (rows of NH * head_size floats
  * or more) and attend to the lengths[b] positions held; with none the row of out is zeros.
- * out: (B, NH * head_size).  Softmax of q.k / sqrt(head_size), as attention_forward.
+ * out: (B, NH * head_size), no part of inp.  Softmax of q.k / sqrt(head_size), as
+ * attention_forward.
  * weights_in, weights_out (both or neither; may be the same array): (B, kv_heads, max_pages *
  * page_size) accumulated attention weights, for kv_evict_paged.  weights_out[b][h][i] becomes
  * weights_in[b][h][i] (0 for the position just appended) plus the weight that position i got
  * from the query heads of kv head h together; entries behind the last position are not touched.
- * A sequence that needs a page that does not exist gets NaN (its new row is stored if its own page
- * exists); so does one whose positions do not fit max_pages * page_size, of which nothing is
- * stored and whose weights are not touched.
+ * A sequence that needs a page that does not exist gets NaN, in weights_out too (its new row is
+ * stored if its own page exists).  One whose positions do not fit max_pages * page_size gets NaN
+ * in out; nothing of it is stored and its weights are not touched.
  * workspace: device memory, 256-byte aligned, for the work to be split over the cache's length;
  * attention_decode_paged_workspace gives the bytes that never constrain the split (0: bad
  * arguments).  With less the work is split less, NULL / 0 means not at all, but weights need
