@@ -408,7 +408,7 @@ class PagedCache:
 def _array(t, cache, dtype, shape, what) -> int:
     """Device pointer of a contiguous tensor of that type and shape on the cache's GPU."""
     try:
-        if t.shape == shape and t.dtype is dtype and t.get_device() == cache._device and t.is_contiguous():
+        if t.dtype is dtype and t.shape == shape and t.get_device() == cache._device and t.is_contiguous():
             return t.data_ptr()
     except AttributeError:
         pass

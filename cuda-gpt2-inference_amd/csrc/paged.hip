@@ -103,47 +103,73 @@ struct Pages {
 // A copy, bound by memory: 8 prompts of 129-1023 rows, 12 heads, fp32: 13.5 us = 4.8 TB/s; 4 of
 // 4001-8192 rows, 8 heads of 128, bf16: 62.7 us = 5.0 TB/s (a 2 GiB copy reaches 4.9).  16-bit rows
 // are stored past the caches (12 x 5-496 rows, 20 heads, fp16: 13.8 -> 11.9 us; fp32 gains nothing).
+// The first loads of the row are under way while its place is looked up.
 template <class E, int VEC>
 __global__ __launch_bounds__(256) void kv_store_paged_kernel(Pages pg, const float* __restrict__ inp, int stride,
                                                              const int* __restrict__ starts,
                                                              const int* __restrict__ lengths, int N, int B, int NH) {
+  constexpr int U = 4, STEP = 64 * VEC;  // loads at a time, floats of one
   const int lane = threadIdx.x & 63;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (r >= N) return;
-  int b = -1;
+  const int HS = pg.head_size, half = pg.kv_heads * HS;
+  const float* src = inp + (size_t)r * stride + (size_t)NH * HS;
+  typedef float In __attribute__((ext_vector_type(VEC)));
+  In x[U];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = min(i0 + u * STEP + lane * VEC, 2 * half - VEC);
+      if constexpr (VEC == 4)
+        x[u] = __builtin_nontemporal_load(reinterpret_cast<const In*>(src + i));
+      else
+        x[u][0] = src[i];
+    }
+  };
+  load(0);
+  int b = -1, begin = 0, n = 0;
   for (int i = 0; i <= B; i += 64) {
-    const bool begun = i + lane <= B && starts[i + lane] <= r;
-    const unsigned long long m = __ballot(begun);
-    b += __popcll(m);
+    const int mine = min(i + lane, B);
+    const int start = starts[mine], held = lengths[min(mine, B - 1)];
+    const unsigned long long m = __ballot(i + lane <= B && start <= r);
+    const int before = __popcll(m);
+    if (before > 0) {
+      begin = __builtin_amdgcn_readlane(start, before - 1);
+      n = __builtin_amdgcn_readlane(held, before - 1);
+    }
+    b += before;
     if (m != ~0ull) break;
   }
-  if (b < 0 || b >= B || starts[b] > r || starts[b + 1] <= r) return;  // in front of the first row or behind the last
-  const int n = lengths[b];
-  const long long pos = (long long)n + (r - starts[b]);
+  // in front of the first row or behind the last; starts that do not ascend are nobody's either
+  if (b < 0 || b >= B || begin > r || starts[b + 1] <= r) return;
+  const long long pos = (long long)n + (r - begin);
   if (n < 0 || pos >= pg.capacity) return;
-  const int HS = pg.head_size, half = pg.kv_heads * HS;
   bool ok = true;
   const unsigned row0 = pg.row(b, 0, (int)pos, ok);
   if (!ok) return;
-  const float* src = inp + (size_t)r * stride + (size_t)NH * HS;
-  for (int i = lane * VEC; i < 2 * half; i += 64 * VEC) {
-    const bool value = i >= half;
-    const int c = value ? i - half : i;
-    const int head = c / HS, d = c - head * HS;
-    E* to = (E*)(value ? pg.values : pg.keys) + ((size_t)row0 + (size_t)head * pg.divide.size) * HS + d;
-    if constexpr (VEC == 4) {
-      typedef unsigned Words __attribute__((ext_vector_type(sizeof(E))));
-      const f32x4 x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(src + i));
-      struct Four {
-        E e[4];
-      };
-      const Words y = __builtin_bit_cast(Words, (Four{{narrow<E>(x[0]), narrow<E>(x[1]), narrow<E>(x[2]), narrow<E>(x[3])}}));
-      if constexpr (sizeof(E) == 2)
-        __builtin_nontemporal_store(y, reinterpret_cast<Words*>(to));
-      else
-        *reinterpret_cast<Words*>(to) = y;
-    } else {
-      to[0] = narrow<E>(src[i]);
+  for (int i0 = 0; i0 < 2 * half; i0 += U * STEP) {
+    if (i0 > 0) load(i0);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int i = i0 + u * STEP + lane * VEC;
+      if (i >= 2 * half) break;
+      const bool value = i >= half;
+      const int c = value ? i - half : i;
+      const int head = c / HS, d = c - head * HS;
+      E* to = (E*)(value ? pg.values : pg.keys) + ((size_t)row0 + (size_t)head * pg.divide.size) * HS + d;
+      if constexpr (VEC == 4) {
+        typedef unsigned Words __attribute__((ext_vector_type(sizeof(E))));
+        struct Four {
+          E e[4];
+        };
+        const Four y{{narrow<E>(x[u][0]), narrow<E>(x[u][1]), narrow<E>(x[u][2]), narrow<E>(x[u][3])}};
+        if constexpr (sizeof(E) == 2)
+          __builtin_nontemporal_store(__builtin_bit_cast(Words, y), reinterpret_cast<Words*>(to));
+        else
+          *reinterpret_cast<Words*>(to) = __builtin_bit_cast(Words, y);
+      } else {
+        to[0] = narrow<E>(x[u][0]);
+      }
     }
   }
 }
