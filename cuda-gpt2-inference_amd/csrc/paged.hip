@@ -101,7 +101,7 @@ struct Pages {
 // One wave per row of the prompts: it finds the row's sequence by counting the starts that are
 // not behind it, 64 at a time, and moves the row's keys and values, VEC floats per lane and step.
 // A copy, bound by memory: 8 prompts of 129-1023 rows, 12 heads, fp32: 13.5 us = 4.8 TB/s; 4 of
-// 4001-8192 rows, 8 heads of 128, bf16: 62.7 us = 5.0 TB/s (a 2 GiB copy reaches 4.9).  16-bit rows
+// 4001-8192 rows, 8 heads of 128, bf16: 57.8 us = 5.4 TB/s (a 2 GiB copy reaches 4.9).  16-bit rows
 // are stored past the caches (12 x 5-496 rows, 20 heads, fp16: 13.8 -> 11.9 us; fp32 gains nothing).
 // The first loads of the row are under way while its place is looked up.
 template <class E, int VEC>
@@ -184,26 +184,20 @@ struct AttendPaged {
   float* weights_out;
   // workspace, where the work is split or weights are asked for
   unsigned* counters;  // (B, kv_heads, chunks) ranges that have arrived: zero between calls
-  float* part_o;       // (B, NH, S, part_stride) unnormalised outputs of the ranges
-  float* part_ml;      // (B, NH, S, 2) their maxima and sums, in the exponent's base-2 scale
+  float* part_o;       // (kv_heads, chunks, slots, part_heads, part_stride) unnormalised outputs of the ranges
+  float* part_ml;      // (kv_heads, chunks, slots, part_heads, 2) their maxima and sums, in the exponent's base-2 scale
   float* joined;       // (B, NH, 2) the whole row's
   float* scores;       // (B, NH, score_stride) base-2 scores
   int B, NH, G, chunks;  // G query heads per kv head, in `chunks` groups of at most GQ
-  int stride, S, min_range, append;  // at most S ranges, of at least min_range positions
-  int weigh_here;  // weights by the same workgroup (S == 1, chunks == 1)
-  int part_stride, score_stride;
+  int stride, append;
+  int slots, min_range;  // workgroups per kv head and chunk: B, or more, for ranges of at least min_range positions
+  int weigh_here;        // weights by the same workgroup (no splitting, one chunk)
+  int part_heads, part_stride, score_stride;
   float scale_log2e;
 };
 
-constexpr int kMaxRanges = 256;
 constexpr int kCounterStride = 32;  // a cache line each: counters that share one are counted one after the other
-
-// How the n positions held by a sequence are dealt to at most S workgroups.
-__device__ __forceinline__ int range_of(int n, int S, int min_range) {
-  const int ranges = max(1, min(S, n / min_range));  // none of them small
-  return ((n + ranges - 1) / ranges + 63) & ~63;
-}
-__device__ __forceinline__ int ranges_of(int n, int range) { return n <= range ? 1 : (n + range - 1) / range; }
+constexpr int kMostSplit = 256;     // sequences whose lengths a wave looks through, four per lane
 
 // exp2(s - above(m)) where m is the running maximum: a maximum of -inf (nothing seen, or only
 // scores of -inf) counts as 0, so that such scores weigh 0 instead of NaN.
@@ -211,45 +205,150 @@ __device__ __forceinline__ float above(float m) { return m == -INFINITY ? 0.f : 
 
 // What one workgroup is to do.
 struct Range {
-  int b, kvh, hc, s;         // sequence, kv head, chunk of its query heads, range
+  int b, kvh, hc;            // sequence, kv head, chunk of its query heads
   int head0, heads;          // the chunk's query heads
-  int n, ranges, p0, p1;     // positions held, ranges they are dealt to, this range
-  bool adds;                 // the new row belongs to this range
+  int n, ranges, s, first;   // positions held, ranges they are dealt to, this one, the slot of the first
+  int p0, p1;                // this range
+  bool adds;                 // the new row belongs to it
 };
 
-__device__ __forceinline__ void take_place(const AttendPaged& a, int GQ, Range& w) {
-  int id = blockIdx.x;
-  w.s = id % a.S;
-  id /= a.S;
-  w.hc = id % a.chunks;
-  id /= a.chunks;
-  w.kvh = id % a.pg.kv_heads;
-  w.b = id / a.pg.kv_heads;
-  w.head0 = w.kvh * a.G + w.hc * GQ;
-  w.heads = min(GQ, a.G - w.hc * GQ);
+__device__ __forceinline__ int across_rows(int v) {  // the sum over the lanes 16, 32 and 48 apart
+  const auto h = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  v = (int)(h[0] + h[1]);
+  const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  return (int)(r[0] + r[1]);
+}
+__device__ __forceinline__ int wave_sum_int(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
+  return across_rows(v);
+}
+// The sum of this lane's value and of those in front of it.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
 }
 
-// False where there is nothing (left) to do: unused places, ranges past the last, sequences that
-// do not fit (NaN) or hold nothing (zeros).
+// Ranges of `size` positions that n positions make, at least one; 0 for an unused place (n < 0).
+__device__ __forceinline__ int ranges_of(int n, int size, float inverse) {
+  int q = (int)((float)n * inverse);  // off by one at most: sizes are an even share or more, so q <= slots
+  int rest = n - q * size;
+  if (rest < 0) {
+    q--;
+    rest += size;
+  }
+  q += rest > size ? 2 : rest > 0 ? 1 : 0;
+  return n < 0 ? 0 : max(q, 1);
+}
+
+// Deals the positions of all sequences to a.slots workgroups in ranges of one size, so that a long
+// sequence gets more of them: slot `slot`'s sequence and range.  The size is the smallest of 16
+// between what an even share would be and what fits whatever the lengths (sum of n / size, and one
+// more range per sequence); four lanes at a time count a size's ranges.  Every wave of every
+// workgroup comes to the same result.  (4 sequences of 1-30000 positions, 4 of 32 heads of 128,
+// bf16: 31.7 us, where every sequence is cut into as many ranges 40.6.)
+__device__ __forceinline__ bool deal(const AttendPaged& a, int slot, int lane, Range& w, int& size) {
+  if (a.B == 1) {
+    w.n = a.lengths[0];
+    const int n = max(w.n, 0);
+    size = max(a.min_range, ((n + a.slots - 1) / a.slots + 63) & ~63);
+    w.ranges = max((n + size - 1) / size, 1);
+    w.b = w.first = 0;
+    w.s = slot;
+    return slot < w.ranges;
+  }
+  const int per = (a.B + 63) >> 6, lanes = (a.B + per - 1) / per, most = a.pg.capacity - a.append;
+  int held[4], n[4], places = 0;  // `per` sequences in this lane; one that does not fit is a range of nothing
+#pragma unroll
+  for (int k = 0; k < 4; k++) held[k] = k < per ? a.lengths[min(lane * per + k, a.B - 1)] : -1;
+  float total = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    if (k >= per || lane * per + k >= a.B) held[k] = -1;
+    n[k] = held[k] > most ? 0 : held[k];
+    places += __popcll(__ballot(n[k] >= 0));
+    total += (float)max(n[k], 0);
+  }
+  total = wave_sum(total);
+  if (places == 0) return false;
+  const float even = total / (float)a.slots, safe = total / (float)(a.slots - places) * 1.0001f + 1.f;
+  const float share = even + (safe - even) * (float)(lane & 15) * (1.f / 15.f);
+  const int mine = max(a.min_range, ((int)fminf(share, 1073741824.f) + 64) & ~63);
+  const float inverse = 1.f / (float)mine;
+  int count = 0;
+  for (int j = 0; j < lanes; j += 4)
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if (k < per) count += ranges_of(__shfl(n[k], j + (lane >> 4), 64), mine, inverse);
+  count = across_rows(count);
+  const unsigned fits = (unsigned)__ballot(count <= a.slots) & 0xffffu;  // the last one always does
+  size = __builtin_amdgcn_readlane(mine, fits ? __builtin_ctz(fits) : 15);
+  const float by = 1.f / (float)size;
+  int c[4], sum = 0;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    c[k] = ranges_of(n[k], size, by);
+    sum += c[k];
+  }
+  const int upto = wave_scan(sum);
+  const int who = __popcll(__ballot(upto <= slot));
+  if (who == 64) return false;
+  int left = slot - __builtin_amdgcn_readlane(upto - sum, who);
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int ck = __builtin_amdgcn_readlane(c[k], who);
+    if (left >= 0 && left < ck) {
+      w.b = who * per + k;
+      w.n = __builtin_amdgcn_readlane(held[k], who);
+      w.ranges = ck;
+      w.s = left;
+      w.first = slot - left;
+      left = -1;
+    } else if (left >= 0) {
+      left -= ck;
+    }
+  }
+  return true;
+}
+
+// False where there is nothing (left) to do: unused places, slots past the last range, sequences
+// that do not fit (NaN) or hold nothing (zeros).
 template <int W>
-__device__ __forceinline__ bool take_range(const AttendPaged& a, int tid, Range& w) {
-  w.n = a.lengths[w.b];
+__device__ __forceinline__ bool take_range(const AttendPaged& a, int GQ, int tid, Range& w) {
+  const int per = a.pg.kv_heads * a.chunks;
+  const int slot = blockIdx.x / per, rest = blockIdx.x - slot * per;
+  w.kvh = rest / a.chunks;
+  w.hc = rest - w.kvh * a.chunks;
+  w.head0 = w.kvh * a.G + w.hc * GQ;
+  w.heads = min(GQ, a.G - w.hc * GQ);
+  int size = 0x7fffffff;
+  if (a.slots > a.B) {
+    if (!deal(a, slot, tid & 63, w, size)) return false;
+  } else {
+    w.b = w.first = slot;
+    w.ranges = 1;
+    w.s = 0;
+    w.n = a.lengths[slot];
+  }
   if (w.n < 0) return false;
   const bool too_long = w.n > a.pg.capacity - a.append;
   if (too_long || w.n + a.append == 0) {
-    if (w.s == 0) {
-      const float fill = too_long ? __builtin_nanf("") : 0.f;
-      for (int i = tid; i < w.heads * a.pg.head_size; i += W * kWave)
-        a.out[((size_t)w.b * a.NH + w.head0) * a.pg.head_size + i] = fill;
-    }
+    const float fill = too_long ? __builtin_nanf("") : 0.f;
+    for (int i = tid; i < w.heads * a.pg.head_size; i += W * kWave)
+      a.out[((size_t)w.b * a.NH + w.head0) * a.pg.head_size + i] = fill;
     return false;
   }
-  const int range = range_of(w.n, a.S, a.min_range);
-  w.ranges = ranges_of(w.n, range);
-  w.p0 = w.s * range;
-  w.p1 = min(w.n, w.p0 + range);
+  w.p0 = w.s == 0 ? 0 : w.s * size;
+  w.p1 = w.s == w.ranges - 1 ? w.n : w.p0 + size;
   w.adds = a.append && w.s == w.ranges - 1;
-  return w.s < w.ranges;
+  return true;
 }
 
 // What the waves of a workgroup hand each other: per wave and head the unnormalised output, the
@@ -329,8 +428,9 @@ __device__ __forceinline__ void finish(const AttendPaged& a, const Range& w, int
   constexpr int THREADS = W * kWave;
   const int HS = a.pg.head_size, HP4 = a.part_stride >> 2;
   const size_t bh0 = (size_t)w.b * a.NH + w.head0;
-  const Bypass parts(a.part_o + (w.ranges > 1 ? bh0 * a.S * a.part_stride : 0),
-                     w.ranges > 1 ? (size_t)w.heads * a.S * a.part_stride : 0);
+  const size_t part0 = w.ranges > 1 ? ((size_t)(w.kvh * a.chunks + w.hc) * a.slots + w.first) * a.part_heads : 0;
+  const Bypass parts(a.part_o + part0 * a.part_stride, w.ranges > 1 ? (size_t)w.ranges * a.part_heads * a.part_stride : 0);
+  unsigned long long* const part_ml = reinterpret_cast<unsigned long long*>(a.part_ml) + part0;
   __syncthreads();
   for (int i = tid; i < w.heads * HP4; i += THREADS) {
     const int g = i / HP4, d = (i - g * HP4) * 4;
@@ -366,11 +466,11 @@ __device__ __forceinline__ void finish(const AttendPaged& a, const Range& w, int
         meet.sum[g] = sum;
       }
     } else {
-      parts.store4((g * a.S + w.s) * a.part_stride + d, acc);
+      const int at = w.s * a.part_heads + g;
+      parts.store4(at * a.part_stride + d, acc);
       if (d == 0) {
         const unsigned long long both = (unsigned long long)__builtin_bit_cast(unsigned, sum) << 32 | __builtin_bit_cast(unsigned, top);
-        __hip_atomic_store(reinterpret_cast<unsigned long long*>(a.part_ml) + (bh0 + g) * a.S + w.s, both, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(part_ml + at, both, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
   }
@@ -395,7 +495,6 @@ __device__ __forceinline__ void finish(const AttendPaged& a, const Range& w, int
   for (int i0 = 0; i0 < w.heads * HP4; i0 += per) {
     const int i = min(i0 + (tid & (per - 1)), w.heads * HP4 - 1);
     const int g = i / HP4, d = (i - g * HP4) * 4;
-    const unsigned long long* ml = reinterpret_cast<const unsigned long long*>(a.part_ml) + (bh0 + g) * a.S;
     float m = -INFINITY, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = slice; s0 < w.ranges; s0 += MOST * slices) {
@@ -407,8 +506,9 @@ __device__ __forceinline__ void finish(const AttendPaged& a, const Range& w, int
         x[u] = 0;
         p[u] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (s < w.ranges) {
-          x[u] = __hip_atomic_load(ml + s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          p[u] = parts.load4((g * a.S + s) * a.part_stride + d);
+          const int at = s * a.part_heads + g;
+          x[u] = __hip_atomic_load(part_ml + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          p[u] = parts.load4(at * a.part_stride + d);
         }
       }
       float mu[MOST], top = m;
@@ -544,7 +644,7 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_kernel(const AttendP
   const int sub = lane & (LPR - 1), rg = lane / LPR;
   const int HS = a.pg.head_size;
   Range w;
-  take_place(a, GQ, w);
+  if (!take_range<W>(a, GQ, tid, w)) return;
   // element j of this lane's part of a row
   auto at = [&](int j) { return SCALAR ? sub + 64 * j : sub * VEC + j; };
   const bool live = SCALAR || sub * VEC < HS;  // lanes behind the row's end read its last piece and count for nothing
@@ -565,7 +665,6 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_kernel(const AttendP
       }
     }
   }
-  if (!take_range<W>(a, tid, w)) return;
   bool ok = true;
   const int p1 = w.p1;
   int t = w.p0 + wave * TILE;
@@ -822,7 +921,7 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const 
   const int col = lane & 15, quad = lane >> 4;
   const int HS = a.pg.head_size;
   Range w;
-  take_place(a, GQ, w);
+  if (!take_range<W>(a, GQ, tid, w)) return;
   // queries of head col, channels 4 PER j + PER quad + e
   f32x4 raw[KS][PER / 4];
   {
@@ -833,7 +932,6 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const 
       for (int e = 0; e < PER; e += 4)
         raw[j][e / 4] = *reinterpret_cast<const f32x4_any*>(src + min(4 * PER * j + PER * quad + e, HS - 4));
   }
-  if (!take_range<W>(a, tid, w)) return;
   bool ok = true;
   const int p1 = w.p1;
   int t = w.p0 + wave * TILE;
@@ -1156,17 +1254,6 @@ __global__ __launch_bounds__(kWeighPositions) void attention_paged_weights_kerne
 __device__ __forceinline__ unsigned rank_of(float w) {
   const unsigned u = __builtin_bit_cast(unsigned, w + 0.0f);
   return w != w ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-}
-
-__device__ __forceinline__ int wave_sum_int(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);
-  const auto h = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
-  v = (int)(h[0] + h[1]);
-  const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
-  return (int)(r[0] + r[1]);
 }
 
 // base + the set bits of m in front of this lane's
@@ -1524,7 +1611,7 @@ static void launch_store(const Pages& pg, const float* inp, int stride, const in
 // Which kernel a problem takes, and how it is cut up.
 struct AttendPlan {
   bool rows16, matrix, deep;
-  int gq, chunks, S, min_range, waves;
+  int gq, chunks, slots, min_range, waves;
 };
 
 static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
@@ -1537,16 +1624,18 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
   const long long groups = (long long)B * c->kv_heads * p.chunks;
   const long long capacity = (long long)c->max_pages * c->page_size, row_bytes = 2LL * c->head_size * type_bytes(c->type);
   const long long each = capacity * row_bytes;  // of keys and values, per group
-  // One workgroup of eight waves per compute unit, or, where that would leave many units idle and
-  // there is much to do, two that follow each other or share it: a split costs 3-4 us (parts to
-  // memory, the counter, parts back), so that short caches are left whole.  A range is worth a
-  // workgroup from 64 KB on.  Beyond 512 groups workgroups follow each other and nothing is split.
+  // As many workgroups as compute units, or, where that is less than two per sequence, there is
+  // much to do and whole sequences would not fill the units evenly, twice as many.  A split costs
+  // 3-4 us (parts to memory, the counter, parts back), so that short caches are left whole; a
+  // range is worth a workgroup from 64 KB on.
   p.min_range = (int)((65536 / row_bytes + 63) & ~63LL);
   if (p.min_range < 128) p.min_range = 128;
-  long long S = groups <= 256 ? 256 / groups : 0;
-  if (S == 0 || (groups * S < 205 && each / S >= 768 * 1024)) S = 512 / groups;
-  if (S > capacity / p.min_range) S = capacity / p.min_range;
-  if (groups * kCounterStride * 4 > GPT2HIP_PAGED_COUNTER_BYTES) S = 1;
+  const long long per = (long long)c->kv_heads * p.chunks, ranges = capacity / p.min_range;  // ranges of a sequence, at most
+  long long slots = 256 / per;
+  if (slots < 2 * B) slots = each >= 768 * 1024 && (groups < 205 || groups > 256) ? 512 / per : 0;
+  if (slots > B * ranges) slots = B * ranges;
+  if (B > kMostSplit || groups * kCounterStride * 4 > GPT2HIP_PAGED_COUNTER_BYTES) slots = 0;
+  p.slots = slots > B ? (int)slots : B;
   // Four waves instead of eight for many short caches (64 sequences of 12 heads, bf16, up to 100
   // positions: 7.0 against 9.3 us; 64 of 16 heads of 128 channels, up to 2000: 135 against 130)
   // and where eight would take all of a unit's registers: the matrix kernel from 257 groups on
@@ -1556,21 +1645,22 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
   p.waves = 8;
   if (!p.rows16 || (groups > 512 && each < 768 * 1024)) p.waves = 4;
   if (p.matrix && (groups > 256 || (capacity <= 128 && type_bytes(c->type) == 2) || c->head_size > 128)) p.waves = 4;
-  p.S = (int)(S < 1 ? 1 : S > kMaxRanges ? kMaxRanges : S);
   // one workgroup per compute unit with much to do: twice the loads under way (16 sequences of 12
   // heads, fp32, up to 1024 positions: 15.8 -> 15.0 us; short ranges would leave waves idle)
-  p.deep = groups * p.S <= 256 && each / p.S >= 256 * 1024;
+  p.deep = (long long)p.slots * c->kv_heads * p.chunks <= 256 && each * B / p.slots >= 256 * 1024;
   return p;
 }
 
 // What a call puts into the workspace behind the counters.
 struct AttendSpace {
   size_t part, ml, joined, scores, total;  // offsets in floats
-  AttendSpace(int B, int NH, int part_stride, int score_stride, int S, bool weights) {
+  AttendSpace(const AttendPlan& p, int B, int NH, int KVH, int part_stride, int score_stride, int slots, bool weights) {
     const size_t rows = (size_t)B * NH;
+    const int G = NH / KVH;
+    const size_t parts = slots > B ? (size_t)slots * KVH * p.chunks * (p.gq < G ? p.gq : G) : 0;
     part = 0;
-    ml = part + (S > 1 ? rows * S * part_stride : 0);
-    joined = ml + (S > 1 ? rows * S * 2 : 0);
+    ml = part + parts * part_stride;
+    joined = ml + parts * 2;
     scores = (joined + (weights ? rows * 2 : 0) + 3) & ~(size_t)3;
     total = scores + (weights ? rows * score_stride : 0);
   }
@@ -1654,7 +1744,8 @@ size_t attention_decode_paged_workspace(const GPT2PagedCache* cache, int B, int 
   Pages pg;
   if (check_cache("attention_decode_paged_workspace", cache, pg)) return 0;
   if (B < 1 || NH < 1 || NH % pg.kv_heads != 0) return 0;
-  const AttendSpace space(B, NH, (pg.head_size + 3) & ~3, (pg.capacity + 63) & ~63, plan_attend(cache, B, NH).S, weights);
+  const AttendPlan plan = plan_attend(cache, B, NH);
+  const AttendSpace space(plan, B, NH, pg.kv_heads, (pg.head_size + 3) & ~3, (pg.capacity + 63) & ~63, plan.slots, weights);
   return GPT2HIP_PAGED_COUNTER_BYTES + space.total * sizeof(float);
 }
 
@@ -1691,16 +1782,17 @@ int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const
   a.part_stride = (HS + 3) & ~3;
   a.score_stride = (a.pg.capacity + 63) & ~63;
   a.scale_log2e = (1.0f / sqrtf((float)HS)) * 1.4426950408889634f;
+  a.part_heads = plan.gq < a.G ? plan.gq : a.G;
   // as many ranges as the workspace holds
   const size_t room = workspace && workspace_bytes > GPT2HIP_PAGED_COUNTER_BYTES
                           ? (workspace_bytes - GPT2HIP_PAGED_COUNTER_BYTES) / sizeof(float) : 0;
-  auto space = [&](int S) { return AttendSpace(B, NH, a.part_stride, a.score_stride, S, weights); };
-  while (plan.S > 1 && space(plan.S).total > room) plan.S--;
-  const AttendSpace use = space(plan.S);
+  auto space = [&](int slots) { return AttendSpace(plan, B, NH, KVH, a.part_stride, a.score_stride, slots, weights); };
+  while (plan.slots > B && space(plan.slots).total > room) plan.slots--;
+  const AttendSpace use = space(plan.slots);
   if (use.total > room)
     return fail(GPT2HIP_EINVAL, "attention_decode_paged: weights need a workspace of at least %zu bytes, got %zu",
                 GPT2HIP_PAGED_COUNTER_BYTES + use.total * sizeof(float), workspace_bytes);
-  a.S = plan.S;
+  a.slots = plan.slots;
   a.min_range = plan.min_range;
   a.counters = (unsigned*)workspace;
   float* at = workspace ? (float*)((char*)workspace + GPT2HIP_PAGED_COUNTER_BYTES) : nullptr;
@@ -1708,8 +1800,8 @@ int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const
   a.part_ml = at + use.ml;
   a.joined = weights ? at + use.joined : nullptr;
   a.scores = weights ? at + use.scores : nullptr;
-  a.weigh_here = weights && a.S == 1 && a.chunks == 1;
-  const long long blocks = (long long)B * KVH * a.chunks * a.S;
+  a.weigh_here = weights && a.slots == B && a.chunks == 1;
+  const long long blocks = (long long)a.slots * KVH * a.chunks;
   const long long weighs = (long long)B * KVH * ((a.pg.capacity + kWeighPositions - 1) / kWeighPositions);
   if (blocks > 0x7fffffffLL || weighs > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "attention_decode_paged: grid too large");
   if (cache->type == GPT2HIP_F32)

@@ -68,9 +68,11 @@ class Case:
             n = max(n, 0)
             k = (torch.randn((KVH, n, HS), generator=g) * keys_std).to(self.kind)
             v = torch.randn((KVH, n, HS), generator=g).to(self.kind)
-            for i in range(min(n, self.cap)):
-                self.keys[order[b, i // page], :, i % page] = k[:, i]
-                self.values[order[b, i // page], :, i % page] = v[:, i]
+            m, used = min(n, self.cap), -(-min(n, self.cap) // page)
+            for pages, rows in ((self.keys, k), (self.values, v)):
+                whole = torch.full((KVH, used * page, HS), float("nan"), dtype=self.kind)
+                whole[:, :m] = rows[:, :m]
+                pages[order[b, :used]] = whole.view(KVH, used, page, HS).transpose(0, 1)
             self.k64.append(k.double())
             self.v64.append(v.double())
         self.inp = torch.randn((B, (NH + 2 * KVH) * HS), generator=g)
@@ -209,6 +211,21 @@ def test_attend_every_form_of_the_kernels(kind, B, NH, KVH, HS, top, weights):
     """Sizes on both sides of every line that the plan of a call draws."""
     say(f"attend {kind} B={B} NH={NH} KVH={KVH} HS={HS} top={top}")
     check_attend(Case(B + HS, kind, B, NH, KVH, HS, 16, spread(B, top), top + 1), weights=weights)
+
+
+@pytest.mark.parametrize("append", [True, False])
+@pytest.mark.parametrize("B,NH,KVH,cap,lengths", [
+    (3, 2, 2, 4000, [4000, 0, 700]), (5, 1, 1, 6000, [6000, 1, -1, 5999, 2500]), (2, 8, 1, 5000, [-1, -1]),
+    (6, 4, 4, 2000, [0, 0, 0, 0, 0, 0]), (4, 6, 2, 3000, [3001, 9000, 2999, 10]),
+    (64, 1, 1, 4000, None), (65, 1, 1, 4000, None), (130, 2, 1, 2000, None), (200, 1, 1, 3200, None),
+])
+def test_attend_deals_positions_to_workgroups(B, NH, KVH, cap, lengths, append):
+    """Sequences of every length under one plan: a few to three hundred ranges, one to four sequences
+    per lane that looks through the lengths, unused places, empty and oversized sequences among them."""
+    say(f"deal B={B} NH={NH} KVH={KVH} cap={cap} append={append}")
+    for kind in ("f16", "f32") if B < 60 else ("f16",):
+        c = Case(B + NH, kind, B, NH, KVH, 64, 16, lengths or spread(B, cap), cap, keys_std=0.5)
+        check_attend(c, append=append, weights=B % 2 == 0)
 
 
 @pytest.mark.parametrize("page", [1, 3, 16, 24, 128, 1000])
