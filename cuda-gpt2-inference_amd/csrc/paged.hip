@@ -1289,23 +1289,33 @@ struct Evict {
 
 // Which of the `older` first positions stay: the `want` (0 < want < older) of largest weight w,
 // for each of which put(place, position) is called.  A workgroup of WAVES waves, all of it.
-// The smallest rank that stays is found two bits at a time by counting how many ranks go each of
-// the four ways: sums of integers, the same on every run.  Once few ranks are left that could be
-// it, they are listed in LDS and the rest is not looked at again until the end; the search ends
-// early where a candidate is reached by exactly as many ranks as are wanted.  A wave owns
-// consecutive positions, so that the places in the output follow from counts alone.  R ranks per
-// thread are kept in registers; R = 0: any length, read again for every count.
+// The first 10 or 12 bits of the smallest rank that stays come from counts in LDS of how many
+// ranks begin with each value (before, two bits at a time from the start: 4 x 32000 weights, 8
+// heads, to 3200: 39.8 -> 33.2 us; 13 x 3-31, 12 heads: 8.9 -> 7.8), the others two at a time from
+// how many ranks go each of the four ways: sums of integers, the same on every run.  Once few
+// ranks are left that could be it, they are listed in LDS and the rest is not looked at again
+// until the end; the search ends early where a candidate is reached by exactly as many ranks as
+// are wanted.  A wave owns consecutive positions, so that the places in the output follow from
+// counts alone.  R ranks per thread are kept in registers; R = 0: any length, read again for
+// every count (200000 weights, 4 heads, to 20000: 147 us).
 template <int WAVES, int R, class Put>
 __device__ __forceinline__ void pick(const float* __restrict__ w, int older, int want, int tid, Put put) {
   constexpr int THREADS = WAVES * kWave;
   constexpr bool LISTS = R == 0 || R * THREADS > 2 * kFew;
   constexpr int FEW = LISTS ? kFew / THREADS : 1;
+  constexpr int BITS = WAVES == 16 ? 12 : 10, BINS = 1 << BITS;
+  static_assert(BINS == 4 * THREADS, "four bins per thread");
   __shared__ unsigned list[LISTS ? kFew : 1];
-  __shared__ int counts[2][WAVES][3], waves[2][WAVES], listed;
+  constexpr int COPIES = 4;
+  __shared__ __align__(16) int bins[COPIES * BINS];
+  __shared__ int counts[2][WAVES][3], waves[2][WAVES], chosen[3], listed;
   const int lane = tid & 63, wave = tid >> 6;
   if (tid == 0) listed = 0;
-  const int span = R ? 64 * R : ((older + WAVES - 1) / WAVES + 63) & ~63;
-  const int first = wave * span, groups = R ? R : span / 64;
+#pragma unroll
+  for (int k = 0; k < COPIES; k++) *reinterpret_cast<int4*>(bins + 4 * (tid + k * THREADS)) = make_int4(0, 0, 0, 0);
+  constexpr int AHEAD = 8;  // loads under way, where nothing is kept
+  const int span = R ? 64 * R : (older + WAVES * AHEAD * 64 - 1) / (WAVES * AHEAD * 64) * AHEAD * 64;
+  const int first = wave * span;
   unsigned rank[R ? R : 1];
   if constexpr (R > 0) {
     float x[R];
@@ -1320,10 +1330,12 @@ __device__ __forceinline__ void pick(const float* __restrict__ w, int older, int
 #pragma unroll
       for (int r = 0; r < R; r++) f(r, rank[r]);
     } else {
-#pragma unroll 8
-      for (int r = 0; r < groups; r++) {
-        const int i = first + r * 64 + lane;
-        f(r, i < older ? rank_of(w[i]) : 0u);
+      for (int r0 = 0; r0 < span / 64; r0 += AHEAD) {
+        float x[AHEAD];
+#pragma unroll
+        for (int r = 0; r < AHEAD; r++) x[r] = w[min(first + (r0 + r) * 64 + lane, older - 1)];
+#pragma unroll
+        for (int r = 0; r < AHEAD; r++) f(r0 + r, first + (r0 + r) * 64 + lane < older ? rank_of(x[r]) : 0u);
       }
     }
   };
@@ -1331,9 +1343,58 @@ __device__ __forceinline__ void pick(const float* __restrict__ w, int older, int
   bool from_list = false;
   __syncthreads();
 
-  unsigned low = 0u;            // at least `want` ranks reach it ...
-  int reach = older, over = 0;  // ... this many; and this many are too large to be the one sought
-  for (int step = 0; step < 16 && reach != want; step++) {
+  // How many ranks begin with each value of BITS bits, in COPIES counts, so that equal ones wait
+  // less for each other (32000 equal weights: 68 us with one, 48 with four).  What is behind the
+  // last position counts as 0, where no weight is.
+  each([&](int, unsigned x) { atomicAdd(&bins[(x >> (32 - BITS)) * COPIES + (lane & (COPIES - 1))], 1); });
+  __syncthreads();
+  {
+    int c[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      c[k] = 0;
+#pragma unroll
+      for (int i = 0; i < COPIES; i++) c[k] += bins[(4 * tid + k) * COPIES + i];
+    }
+    const int sum = c[0] + c[1] + c[2] + c[3], upto = wave_scan(sum);
+    if (lane == 63) waves[0][wave] = upto;
+    __syncthreads();
+    int at_least = span * WAVES - (upto - sum);  // ranks from this thread's bins on
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) at_least -= i < wave ? waves[0][i] : 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (at_least >= want && at_least - c[k] < want) {
+        chosen[0] = 4 * tid + k;
+        chosen[1] = at_least;
+        chosen[2] = at_least - c[k];
+      }
+      at_least -= c[k];
+    }
+  }
+  __syncthreads();
+  unsigned low = (unsigned)chosen[0] << (32 - BITS);  // at least `want` ranks reach it ...
+  int reach = chosen[1], over = chosen[2];  // ... this many; and this many are too large to be the one sought
+  auto to_list = [&](int shift) {
+    if constexpr (LISTS) {
+      if (from_list || reach - over > kFew || reach == want) return;
+      int mine = 0;  // low is above 0 by now, so that nothing behind the last position counts
+      each([&](int, unsigned x) { mine += (x - low) >> shift == 0u; });
+      const int upto = wave_scan(mine);
+      int at = 0;
+      if (lane == 63) at = atomicAdd(&listed, upto);
+      at = __builtin_amdgcn_readlane(at, 63) + upto - mine;
+      each([&](int, unsigned x) {
+        if ((x - low) >> shift == 0u && at < kFew) list[at++] = x;
+      });
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < FEW; k++) few[k] = k * THREADS + tid < min(listed, kFew) ? list[k * THREADS + tid] : 0u;
+      from_list = true;
+    }
+  };
+  to_list(32 - BITS);
+  for (int step = BITS / 2; step < 16 && reach != want; step++) {
     // the four ways the next two bits can go, for ranks that agree with low in front of them
     const int shift = 30 - 2 * step;
     int n1, n2, n3;
@@ -1387,40 +1448,21 @@ __device__ __forceinline__ void pick(const float* __restrict__ w, int older, int
     } else {
       over = c1;
     }
-    if constexpr (LISTS) {
-      if (!from_list && reach - over <= kFew && reach != want) {
-        int mine = 0;
-        each([&](int, unsigned x) { mine += x != 0u && (x - low) >> shift == 0u; });
-        mine = wave_sum_int(mine);
-        if (lane == 0) mine = atomicAdd(&listed, mine);
-        int at = __builtin_amdgcn_readfirstlane(mine);
-        each([&](int, unsigned x) {
-          const bool in = x != 0u && (x - low) >> shift == 0u;
-          const unsigned long long m = __ballot(in);
-          const int to = lanes_before(m, at);
-          if (in && to < kFew) list[to] = x;
-          at += __popcll(m);
-        });
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < FEW; k++) few[k] = k * THREADS + tid < min(listed, kFew) ? list[k * THREADS + tid] : 0u;
-        from_list = true;
-      }
-    }
+    to_list(shift);
   }
 
   // All ranks above low stay, and of its equals as many as there is room for: all of them, where
   // exactly as many as are wanted reach low.
   const bool exact = reach == want;
   int gt = 0, eq = 0;
-  each([&](int, unsigned x) {
-    gt += x >= low;
-    eq += x == low;
-  });
-  gt = wave_sum_int(gt);
-  eq = wave_sum_int(eq);
+  each([&](int, unsigned x) { gt += x >= low; });
+  if (!exact) {
+    each([&](int, unsigned x) { eq += x == low; });
+    eq = wave_sum_int(eq);
+  }
+  gt = wave_sum_int(gt) - eq;
   if (lane == 0) {
-    waves[0][wave] = exact ? gt : gt - eq;
+    waves[0][wave] = gt;
     waves[1][wave] = eq;
   }
   __syncthreads();

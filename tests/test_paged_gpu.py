@@ -747,6 +747,18 @@ def test_evict_ties_beyond_the_registers():
     check_evict(4, "f16", [40000, 39999], 20000, 100, KVH=1, HS=8, page=64, weights=ties)
 
 
+def lowest(B, KVH, cap, g):
+    return torch.where(torch.rand((B, KVH, cap), generator=g) < 0.9, -math.inf, torch.rand((B, KVH, cap), generator=g))
+
+
+@pytest.mark.parametrize("weights", [special, lowest, zeros], ids=lambda f: f.__name__)
+@pytest.mark.parametrize("n,budget", [(1023, 900), (4095, 5), (20001, 15000), (40001, 30000)])
+def test_evict_special_weights_of_every_form(n, budget, weights):
+    """Ranks at both ends of their order, next to what is behind the last position."""
+    say(f"evict special n={n} budget={budget}")
+    check_evict(11, "f16", [n, budget + 6, n - 1], budget, 4, KVH=1, HS=8, page=64, weights=weights)
+
+
 def test_evict_pages_that_do_not_exist():
     check_evict(5, "f32", [300, 300, 300], 100, 10, bad_src=(1, 4), bad_dst=(2, 2))
 
