@@ -255,17 +255,18 @@ __device__ __forceinline__ int ranges_of(int n, int size, float inverse) {
 // workgroup comes to the same result.  (4 sequences of 1-30000 positions, 4 of 32 heads of 128,
 // bf16: 31.7 us, where every sequence is cut into as many ranges 40.6.)
 __device__ __forceinline__ bool deal(const AttendPaged& a, int slot, int lane, Range& w, int& size) {
+  const int most = a.pg.capacity - a.append;  // a sequence that does not fit is a range of nothing
   if (a.B == 1) {
     w.n = a.lengths[0];
-    const int n = max(w.n, 0);
+    const int n = w.n > most ? 0 : max(w.n, 0);
     size = max(a.min_range, ((n + a.slots - 1) / a.slots + 63) & ~63);
     w.ranges = max((n + size - 1) / size, 1);
     w.b = w.first = 0;
     w.s = slot;
     return slot < w.ranges;
   }
-  const int per = (a.B + 63) >> 6, lanes = (a.B + per - 1) / per, most = a.pg.capacity - a.append;
-  int held[4], n[4], places = 0;  // `per` sequences in this lane; one that does not fit is a range of nothing
+  const int per = (a.B + 63) >> 6, lanes = (a.B + per - 1) / per;
+  int held[4], n[4], places = 0;  // `per` sequences in this lane
 #pragma unroll
   for (int k = 0; k < 4; k++) held[k] = k < per ? a.lengths[min(lane * per + k, a.B - 1)] : -1;
   float total = 0.f;
@@ -1548,7 +1549,8 @@ __device__ __forceinline__ void copy_kept(const Evict& e, size_t bh, int b, int 
 // COPY (up to 4096 weights, where a second launch would cost as much as the choice): several
 // workgroups per (sequence, kv head), each of which makes the whole choice and copies its share of
 // the rows.  8 sequences of 900-1024 positions, 12 heads, fp32, to 512: 14.5 us (two launches: 17.9).
-// Alone, 4 of 32768, 8 heads: 25 us on 32 compute units, half of it counting in registers.
+// Alone, 4 of 32768, 8 heads: 20 us on 32 compute units: loading 3.4, first counts 4.5, the list 3,
+// the other bits 3, what stays 4 (the 100 MHz clock's stamps).
 template <int WAVES, int R, bool COPY, int UNIT, bool STREAM>
 __global__ __launch_bounds__(WAVES* kWave) void kv_evict_pick_kernel(const Evict e) {
   constexpr int THREADS = WAVES * kWave;

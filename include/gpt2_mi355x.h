@@ -225,8 +225,9 @@ int matmul_forward_argmax_noalloc_status(int* ids, const float* inp, const float
  * lengths (B, int32, on the device) says how many positions each sequence holds; a negative one
  * marks an unused place in the batch: no page of it is read or written, and its rows of every
  * output stay as they were.  Table entries outside [0, num_pages) are never followed: see each
- * call; nor are entries behind a sequence's last position, which may hold anything.  Nothing is allocated, nothing
- * synchronises, nothing is kept between calls: the calls can be captured in a graph. */
+ * call; nor are entries behind a sequence's last position, which may hold anything.  Nothing is
+ * allocated, nothing synchronises, nothing is kept between calls: the calls can be captured in a
+ * graph. */
 enum { GPT2HIP_F32 = 0, GPT2HIP_F16 = 1, GPT2HIP_BF16 = 2 };
 typedef struct {
   void* keys;       /* (num_pages, kv_heads, page_size, head_size) of `type`, on the device */
