@@ -1658,7 +1658,7 @@ struct AttendPlan {
   int gq, chunks, slots, min_range, waves;
 };
 
-static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
+static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH, bool weights) {
   AttendPlan p;
   const int G = NH / c->kv_heads;
   p.rows16 = rows_by_16(c);
@@ -1669,14 +1669,25 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH) {
   const long long capacity = (long long)c->max_pages * c->page_size, row_bytes = 2LL * c->head_size * type_bytes(c->type);
   const long long each = capacity * row_bytes;  // of keys and values, per group
   // As many workgroups as compute units, or, where that is less than two per sequence, there is
-  // much to do and whole sequences would not fill the units evenly, twice as many.  A split costs
-  // 3-4 us (parts to memory, the counter, parts back), so that short caches are left whole; a
-  // range is worth a workgroup from 64 KB on.
+  // much to do and whole sequences would not fill the units evenly, twice as many.  A range is
+  // worth a workgroup from 64 KB on.
   p.min_range = (int)((65536 / row_bytes + 63) & ~63LL);
   if (p.min_range < 128) p.min_range = 128;
   const long long per = (long long)c->kv_heads * p.chunks, ranges = capacity / p.min_range;  // ranges of a sequence, at most
   long long slots = 256 / per;
-  if (slots < 2 * B) slots = each >= 768 * 1024 && (groups < 205 || groups > 256) ? 512 / per : 0;
+  if (slots < 2 * B) {
+    slots = each >= 768 * 1024 && (groups < 205 || groups > 256) ? 512 / per : 0;
+  } else {
+    // Splitting costs 4 us (parts to memory, the counter, parts back) and, with weights, a second
+    // launch.  A workgroup takes 18 ns for a KB of cache, 27 in the matrix kernel, and all of them
+    // together at least 0.12 ns per KB.  (12 heads, fp32: whole or split, one sequence of 384
+    // positions 6.7 or 8.3 us, of 640 9.2 or 8.4; 8 of 896 13.3 or 15.2, of 1800 23.1 or 21.7,
+    // with weights 25.9 or 25.0.  4 sequences, 8 of 32 heads of 128, bf16: 384 11.3 or 11.9, with
+    // weights 12.4 or 15.3; 640 14.9 or 11.9, with weights 16.0 or 15.3.)
+    const double alone = p.matrix ? 27. : 18., parts = (double)(slots < B * ranges ? slots : B * ranges) / B;
+    const double split = parts > 1. ? alone / parts : alone, together = 0.12 * (double)groups;
+    if ((double)each / 1024. * (alone - (split > together ? split : together)) < (weights ? 5300. : 4000.)) slots = 0;
+  }
   if (slots > B * ranges) slots = B * ranges;
   if (B > kMostSplit || groups * kCounterStride * 4 > GPT2HIP_PAGED_COUNTER_BYTES) slots = 0;
   p.slots = slots > B ? (int)slots : B;
@@ -1788,9 +1799,13 @@ size_t attention_decode_paged_workspace(const GPT2PagedCache* cache, int B, int 
   Pages pg;
   if (check_cache("attention_decode_paged_workspace", cache, pg)) return 0;
   if (B < 1 || NH < 1 || NH % pg.kv_heads != 0) return 0;
-  const AttendPlan plan = plan_attend(cache, B, NH);
-  const AttendSpace space(plan, B, NH, pg.kv_heads, (pg.head_size + 3) & ~3, (pg.capacity + 63) & ~63, plan.slots, weights);
-  return GPT2HIP_PAGED_COUNTER_BYTES + space.total * sizeof(float);
+  size_t most = 0;  // with weights, what a call without them needs too
+  for (int w = 0; w <= (weights != 0); w++) {
+    const AttendPlan plan = plan_attend(cache, B, NH, w);
+    const AttendSpace space(plan, B, NH, pg.kv_heads, (pg.head_size + 3) & ~3, (pg.capacity + 63) & ~63, plan.slots, w);
+    if (space.total > most) most = space.total;
+  }
+  return GPT2HIP_PAGED_COUNTER_BYTES + most * sizeof(float);
 }
 
 int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const float* inp, int inp_stride,
@@ -1811,7 +1826,7 @@ int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const
   if (!out || !inp || !lengths) return fail(GPT2HIP_EINVAL, "attention_decode_paged: null pointer");
   if ((uintptr_t)workspace % 256) return fail(GPT2HIP_EINVAL, "attention_decode_paged: workspace must be 256-byte aligned");
   const bool weights = weights_out != nullptr;
-  AttendPlan plan = plan_attend(cache, B, NH);
+  AttendPlan plan = plan_attend(cache, B, NH, weights);
   a.out = out;
   a.inp = inp;
   a.lengths = lengths;

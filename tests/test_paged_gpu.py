@@ -217,7 +217,8 @@ def test_attend_every_form_of_the_kernels(kind, B, NH, KVH, HS, top, weights):
 @pytest.mark.parametrize("B,NH,KVH,cap,lengths", [
     (3, 2, 2, 4000, [4000, 0, 700]), (5, 1, 1, 6000, [6000, 1, -1, 5999, 2500]), (2, 8, 1, 5000, [-1, -1]),
     (6, 4, 4, 2000, [0, 0, 0, 0, 0, 0]), (4, 6, 2, 3000, [3001, 9000, 2999, 10]),
-    (64, 1, 1, 4000, None), (65, 1, 1, 4000, None), (130, 2, 1, 2000, None), (200, 1, 1, 3200, None),
+    (64, 1, 1, 4000, None), (65, 1, 1, 4000, None), (130, 2, 1, 2000, None), (130, 1, 1, 4000, None),
+    (200, 1, 1, 3200, None),
 ])
 def test_attend_deals_positions_to_workgroups(B, NH, KVH, cap, lengths, append):
     """Sequences of every length under one plan: a few to three hundred ranges, one to four sequences
@@ -226,6 +227,21 @@ def test_attend_deals_positions_to_workgroups(B, NH, KVH, cap, lengths, append):
     for kind in ("f16", "f32") if B < 60 else ("f16",):
         c = Case(B + NH, kind, B, NH, KVH, 64, 16, lengths or spread(B, cap), cap, keys_std=0.5)
         check_attend(c, append=append, weights=B % 2 == 0)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("NH,KVH,HS,page,cap", [
+    (2, 2, 64, 16, 6000), (4, 2, 128, 24, 4000), (3, 1, 80, 1, 5000), (8, 1, 96, 7, 5000), (40, 2, 64, 16, 5000),
+    (5, 1, 33, 16, 6000), (2, 1, 256, 32, 2000), (16, 2, 200, 50, 2500), (1, 1, 8, 16, 30000), (2, 1, 20, 1000, 12000),
+])
+def test_attend_split_forms(kind, NH, KVH, HS, page, cap):
+    """Caches long enough for several ranges per sequence, in every form of the kernels."""
+    say(f"split {kind} NH={NH} KVH={KVH} HS={HS} page={page} cap={cap}")
+    c = Case(NH + HS, kind, 5, NH, KVH, HS, page, [cap, cap - 1, 1, -1, cap // 2 + 3], cap + 1, keys_std=0.5)
+    whole = g2.PAGED_COUNTER_BYTES + 16
+    assert g2.attention_decode_paged_workspace(c.gpu(), 5, NH).nbytes > whole
+    check_attend(c)
+    check_attend(c, append=False, weights=True)
 
 
 @pytest.mark.parametrize("page", [1, 3, 16, 24, 128, 1000])
@@ -369,6 +385,36 @@ def test_attend_pages_that_do_not_exist_give_nan_rows_only():
         for b in (0, 3):
             exp, tol, _, _ = c.expect(b, True)
             assert ((out[b].cpu().double() - exp).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("kind,NH", [("f16", 2), ("f32", 4), ("bf16", 10)])
+def test_attend_split_nan_and_pages_that_do_not_exist(kind, NH):
+    """One range of many sees it: its whole row shows it, in the weights too, and no other row does."""
+    lengths = [4000, 4000, 3999, 4000]
+    c = Case(16, kind, 4, NH, 2, 64, 16, lengths, 4016)
+    c.table[1, 200] = c.keys.shape[0]
+    c.keys[c.table[2, 30], 0, 4, 7] = float("nan")
+    c.table[3, 250] = -1  # the page of the new row
+    cache = c.gpu()
+    ws = g2.attention_decode_paged_workspace(cache, 4, NH, weights=True)
+    out = torch.zeros((4, NH * 64), device="cuda")
+    w = torch.rand((4, 2, c.cap), device="cuda")
+    wo = torch.full_like(w, 7.0)
+    for _ in range(2):
+        g2.attention_decode_paged(out, cache, c.inp.cuda(), c.dl, 4, NH, weights_in=w, weights_out=wo, workspace=ws)
+        bad, badw = torch.isnan(out).cpu(), torch.isnan(wo).cpu()
+        half = NH * 32  # what the heads of the first kv head write
+        for b in range(4):
+            n = lengths[b] + 1
+            both = b in (1, 3)
+            assert bad[b, :half].all() if both or b == 2 else not bad[b, :half].any(), b
+            assert bad[b, half:].all() if both else not bad[b, half:].any(), b
+            assert badw[b, 0, :n].all() if both or b == 2 else not badw[b, 0, :n].any(), b
+            assert badw[b, 1, :n].all() if both else not badw[b, 1, :n].any(), b
+        assert (wo[:, :, 4001:] == 7.0).all()
+        exp, tol, _, _ = c.expect(0, True)
+        assert ((out[0].cpu().double() - exp).abs() <= tol).all()
+    assert not ws[: g2.PAGED_COUNTER_BYTES].any()
 
 
 def test_attend_is_repeatable_and_replays_in_a_graph():
