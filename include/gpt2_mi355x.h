@@ -257,7 +257,9 @@ int kv_store_paged_status(const GPT2PagedCache* cache, const float* inp, int inp
  * 0 .. lengths[b].  append == 0: only the queries of inp are read (rows of NH * head_size floats
  * or more) and attend to the lengths[b] positions held; with none the row of out is zeros.
  * out: (B, NH * head_size), no part of inp.  Softmax of q.k / sqrt(head_size), as
- * attention_forward.
+ * attention_forward.  An infinity among the values gives that infinity in its channel (infinities
+ * of both signs, or a NaN, a NaN) for every query head that weighs it with 2^-126 or more; where
+ * the weight is below, an infinity or a NaN; where it is 0 exactly, from a score of -inf, a NaN.
  * weights_in, weights_out (both or neither; may be the same array): (B, kv_heads, max_pages *
  * page_size) accumulated attention weights, for kv_evict_paged.  weights_out[b][h][i] becomes
  * weights_in[b][h][i] (0 for the position just appended) plus the weight that position i got
