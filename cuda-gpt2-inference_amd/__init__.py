@@ -429,6 +429,16 @@ def _rows(inp, cache, count, floats):
     return inp.data_ptr(), strides[0] if count > 1 else max(strides[0], floats)
 
 
+def _space(workspace, cache):
+    """(pointer, bytes) of a contiguous workspace on the cache's GPU."""
+    if not hasattr(workspace, "get_device") or workspace.get_device() != cache._device:
+        raise TypeError(f"workspace is a tensor on cuda:{cache._device}, got {getattr(workspace, 'dtype', type(workspace))} on "
+                        f"{getattr(workspace, 'device', 'the host')}")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return workspace.data_ptr(), workspace.nbytes
+
+
 def _on_its_gpu(cache, B) -> None:
     """Launchers run on the current device: the cache has to be there, and to list B sequences."""
     if cache._current_device() != cache._device:
@@ -476,7 +486,7 @@ def attention_decode_paged(out, cache, inp, lengths, B, NH, append=True, weights
     if weights_out is not None:
         wout = _array(weights_out, cache, f, (B, cache.kv_heads, cache.capacity), "weights_out")
     if workspace is not None:
-        ws, nbytes = _ptr(workspace), workspace.nbytes
+        ws, nbytes = _space(workspace, cache)
     _check(lib().attention_decode_paged_status(_array(out, cache, f, (B, NH * HS), "out"), cache._ref, rows,
                                                stride, _array(lengths, cache, cache._int, (B,), "lengths"), win, wout, B, NH,
                                                1 if append else 0, ws, nbytes), "attention_decode_paged")

@@ -1,0 +1,70 @@
+"""CPU-only checks of what the paged cache's Python calls refuse and where they allocate, with
+tensors that only claim to lie on a GPU; the library is replaced by a recorder, so nothing runs."""
+import contextlib
+import importlib
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+g2 = importlib.import_module("cuda-gpt2-inference_amd")
+
+
+class OnGpu(torch.Tensor):
+    """A host tensor that says it is on GPU `at`."""
+
+    @staticmethod
+    def of(shape, dtype=torch.float32, at=1):
+        t = torch.zeros(shape, dtype=dtype).as_subclass(OnGpu)
+        t.at = at
+        return t
+
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return self.at
+
+
+class Recorder:
+    """Stands in for the library: takes every call for a good one."""
+
+    def __init__(self, **results):
+        self.calls, self.results = [], results
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return self.results.get(name, 0)
+        return call
+
+
+@pytest.fixture
+def library(monkeypatch):
+    r = Recorder(attention_decode_paged_workspace=g2.PAGED_COUNTER_BYTES + 1024)
+    monkeypatch.setattr(g2, "lib", lambda: r)
+    return r
+
+
+@pytest.fixture
+def cache(monkeypatch, library):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    return g2.PagedCache(OnGpu.of((8, 2, 16, 64)), OnGpu.of((8, 2, 16, 64)), OnGpu.of((2, 4), torch.int32))
+
+
+def step(cache, **other):
+    a = dict(out=OnGpu.of((2, 4 * 64)), cache=cache, inp=OnGpu.of((2, 8 * 64)), lengths=OnGpu.of((2,), torch.int32), B=2, NH=4)
+    a.update(other)
+    g2.attention_decode_paged(**a)
+
+
+def test_a_workspace_on_another_gpu_is_refused(cache, library):
+    step(cache)
+    step(cache, workspace=OnGpu.of((g2.PAGED_COUNTER_BYTES,), torch.uint8))
+    assert [name for name, _ in library.calls] == ["attention_decode_paged_status"] * 2
+    with pytest.raises(TypeError, match="workspace.*cuda:1"):
+        step(cache, workspace=OnGpu.of((g2.PAGED_COUNTER_BYTES,), torch.uint8, at=0))
+    with pytest.raises(TypeError, match="workspace.*cuda:1"):
+        step(cache, workspace=bytearray(g2.PAGED_COUNTER_BYTES))
+    with pytest.raises(ValueError, match="contiguous"):
+        step(cache, workspace=OnGpu.of((2 * g2.PAGED_COUNTER_BYTES,), torch.uint8)[::2])
+    assert len(library.calls) == 2, "a refused call reached the library"
