@@ -19,6 +19,7 @@ class OnGpu(torch.Tensor):
         t.at = at
         return t
 
+    at = 1  # of views
     is_cuda = property(lambda self: True)
 
     def get_device(self):
