@@ -462,12 +462,17 @@ PAGED_COUNTER_BYTES = 65536  # GPT2HIP_PAGED_COUNTER_BYTES
 
 def attention_decode_paged_workspace(cache, B, NH, weights=False):
     """A zero-filled workspace (uint8 CUDA tensor) that never constrains how attention_decode_paged
-    splits the work.  Its first PAGED_COUNTER_BYTES stay zero between calls."""
+    splits the work.  Its first PAGED_COUNTER_BYTES stay zero between calls.  It is allocated and
+    zeroed on the launchers' stream (set_stream), whatever torch's current one is: calls on that
+    stream find it zero, one on another stream has to be ordered behind it."""
     import torch
     n = lib().attention_decode_paged_workspace(cache._ref, B, NH, int(weights))
     if n == 0:
         raise GPT2HipError(f"attention_decode_paged_workspace: bad arguments B={B} NH={NH} kv_heads={cache.kv_heads}")
-    return torch.zeros(n, dtype=torch.uint8, device=cache.keys.device)
+    device = cache.keys.device
+    raw = lib().gpt2hip_get_stream()
+    with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=device) if raw else torch.cuda.default_stream(device)):
+        return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
 def attention_decode_paged(out, cache, inp, lengths, B, NH, append=True, weights_in=None, weights_out=None,

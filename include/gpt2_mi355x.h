@@ -271,8 +271,9 @@ int kv_store_paged_status(const GPT2PagedCache* cache, const float* inp, int inp
  * attention_decode_paged_workspace gives the bytes that never constrain the split (0: bad
  * arguments).  With less the work is split less, NULL / 0 means not at all, but weights need
  * GPT2HIP_PAGED_COUNTER_BYTES and B * NH * (max_pages * page_size + 68) floats.  Its first
- * GPT2HIP_PAGED_COUNTER_BYTES are counters: zero them once (hipMemset) before the first call;
- * every call leaves them zero (zero them again after a launch that did not run to completion).
+ * GPT2HIP_PAGED_COUNTER_BYTES are counters: zero them once (hipMemset) before the first call, on
+ * the call's stream or ordered before it; every call leaves them zero (zero them again after a
+ * launch that did not run to completion).
  * The rest is scratch.  Calls that overlap on one GPU need a workspace each, calls of any sizes
  * one after the other can share one. */
 #define GPT2HIP_PAGED_COUNTER_BYTES 65536u

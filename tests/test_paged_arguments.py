@@ -69,3 +69,26 @@ def test_a_workspace_on_another_gpu_is_refused(cache, library):
     with pytest.raises(ValueError, match="contiguous"):
         step(cache, workspace=OnGpu.of((2 * g2.PAGED_COUNTER_BYTES,), torch.uint8)[::2])
     assert len(library.calls) == 2, "a refused call reached the library"
+
+
+@pytest.mark.parametrize("launchers", [None, 0x5000])
+def test_a_workspace_is_zeroed_on_the_stream_of_the_launchers(cache, library, monkeypatch, launchers):
+    """Its counters have to be zero when the first call's kernel reads them, whatever torch's own
+    current stream has to do before."""
+    library.results["gpt2hip_get_stream"] = launchers
+    order, current = [], ["torch's current stream"]
+
+    @contextlib.contextmanager
+    def stream(s):
+        current.append(s.cuda_stream)
+        yield
+        current.pop()
+
+    monkeypatch.setattr(torch.cuda, "stream", stream)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda raw, device=None: types.SimpleNamespace(cuda_stream=raw))
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: types.SimpleNamespace(cuda_stream=0))
+    zeros = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, **k: (order.append(current[-1]), zeros(*a, **{**k, "device": "cpu"}))[1])
+    space = g2.attention_decode_paged_workspace(cache, 2, 4)
+    assert space.nbytes == g2.PAGED_COUNTER_BYTES + 1024 and not space.any()
+    assert order == [launchers or 0]
