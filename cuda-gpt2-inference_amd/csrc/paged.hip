@@ -1264,23 +1264,29 @@ __global__ __launch_bounds__(W* kWave) void attention_paged_matrix_kernel(const 
 
 constexpr int kWeighPositions = 256;  // positions per workgroup
 
-// The same where the work is split: a thread per position.
-__global__ __launch_bounds__(kWeighPositions) void attention_paged_weights_kernel(const AttendPaged a) {
-  const int per = (a.pg.capacity + kWeighPositions - 1) / kWeighPositions;
-  int id = blockIdx.x;
-  const int i = (id % per) * kWeighPositions + threadIdx.x;
-  id /= per;
-  const int kvh = id % a.pg.kv_heads, b = id / a.pg.kv_heads;
-  const int n = a.lengths[b];
-  if (n < 0 || n > a.pg.capacity - a.append || i >= n + a.append) return;
-  const size_t at = ((size_t)b * a.pg.kv_heads + kvh) * a.pg.capacity + i;
-  const size_t bh = (size_t)b * a.NH + kvh * a.G;
-  const float x = i < n ? a.weights_in[at] : 0.f;
-  float p = 0.f;
+// The same where the work is split: a thread per position.  TURNS: as many workgroups as a launch
+// holds, which take the rest of the `blocks` in further turns (a loop that costs narrower tables
+// 0.3 of 21.4 us: 4 sequences of 5000-9001 positions, 4 of 32 heads of 96, bf16).
+template <bool TURNS>
+__global__ __launch_bounds__(kWeighPositions) void attention_paged_weights_kernel(const AttendPaged a, unsigned blocks) {
+  const unsigned per = (unsigned)(a.pg.capacity + kWeighPositions - 1) / kWeighPositions;
+  unsigned turn = blockIdx.x;
+  do {
+    const unsigned pair = turn / per, kvh = pair % a.pg.kv_heads, b = pair / a.pg.kv_heads;
+    const int i = (int)(turn - pair * per) * kWeighPositions + threadIdx.x;
+    const int n = a.lengths[b];
+    if (n >= 0 && n <= a.pg.capacity - a.append && i < n + a.append) {
+      const size_t at = ((size_t)b * a.pg.kv_heads + kvh) * a.pg.capacity + i;
+      const size_t bh = (size_t)b * a.NH + kvh * a.G;
+      const float x = i < n ? a.weights_in[at] : 0.f;
+      float p = 0.f;
 #pragma unroll 8
-  for (int g = 0; g < a.G; g++)
-    p += __builtin_amdgcn_exp2f(a.scores[(bh + g) * a.score_stride + i] - a.joined[(bh + g) * 2]) / a.joined[(bh + g) * 2 + 1];
-  a.weights_out[at] = x + p;
+      for (int g = 0; g < a.G; g++)
+        p += __builtin_amdgcn_exp2f(a.scores[(bh + g) * a.score_stride + i] - a.joined[(bh + g) * 2]) / a.joined[(bh + g) * 2 + 1];
+      a.weights_out[at] = x + p;
+    }
+    turn += gridDim.x;
+  } while (TURNS && turn < blocks);
 }
 
 // ---- kv_evict_paged -------------------------------------------------------------------------
@@ -1641,6 +1647,9 @@ __global__ __launch_bounds__(256) void kv_evict_copy_kernel(const Evict e) {
 }
 
 // ---- launchers ------------------------------------------------------------------------------
+// A launch holds fewer than 2^32 threads in all; what is beyond is left out without an error.
+static bool too_many(long long blocks, int threads) { return blocks > 0xffffffffLL / threads; }
+
 static size_t type_bytes(int type) { return type == GPT2HIP_F32 ? 4 : 2; }
 
 static int check_cache(const char* name, const GPT2PagedCache* c, Pages& pg) {
@@ -1679,7 +1688,7 @@ static bool rows_by_16(const GPT2PagedCache* c) {
 template <class E>
 static void launch_store(const Pages& pg, const float* inp, int stride, const int* starts, const int* lengths, int N,
                          int B, int NH, bool vec) {
-  const dim3 grid((unsigned)((N + 3) / 4)), block(256);
+  const dim3 grid((unsigned)((N + 3LL) / 4)), block(256);
   if (vec)
     hipLaunchKernelGGL((kv_store_paged_kernel<E, 4>), grid, block, 0, stream(), pg, inp, stride, starts, lengths, N, B, NH);
   else
@@ -1709,7 +1718,7 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH, bool weigh
   if (p.min_range < 128) p.min_range = 128;
   const long long per = (long long)c->kv_heads * p.chunks, ranges = capacity / p.min_range;  // ranges of a sequence, at most
   long long slots = 256 / per;
-  if (slots < 2 * B) {
+  if (slots < 2LL * B) {
     slots = each >= 768 * 1024 && (groups < 205 || groups > 256) ? 512 / per : 0;
   } else {
     // Splitting costs 4 us (parts to memory, the counter, parts back) and, with weights, a second
@@ -1815,6 +1824,7 @@ int kv_store_paged_status(const GPT2PagedCache* cache, const float* inp, int inp
   const long long need = ((long long)NH + 2LL * pg.kv_heads) * pg.head_size;
   if (inp_stride < need)
     return fail(GPT2HIP_EINVAL, "kv_store_paged: rows of %lld floats at a stride of %d", need, inp_stride);
+  if (too_many((N + 3LL) / 4, 256)) return fail(GPT2HIP_EINVAL, "kv_store_paged: grid too large (N=%d rows)", N);
   if (N == 0 || B == 0) return GPT2HIP_OK;
   if (!inp || !starts || !lengths) return fail(GPT2HIP_EINVAL, "kv_store_paged: null pointer");
   const bool vec = pg.head_size % 4 == 0 && inp_stride % 4 == 0 && aligned16(inp) && aligned16(pg.keys) && aligned16(pg.values);
@@ -1896,7 +1906,8 @@ int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const
   a.weigh_here = weights && a.slots == B && a.chunks == 1;
   const long long blocks = (long long)a.slots * KVH * a.chunks;
   const long long weighs = (long long)B * KVH * ((a.pg.capacity + kWeighPositions - 1) / kWeighPositions);
-  if (blocks > 0x7fffffffLL || weighs > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "attention_decode_paged: grid too large");
+  if (too_many(blocks, plan.waves * kWave) || weighs > 0x7fffffffLL)
+    return fail(GPT2HIP_EINVAL, "attention_decode_paged: grid too large (B=%d, NH=%d)", B, NH);
   if (cache->type == GPT2HIP_F32)
     launch_attend<float>(a, plan, (unsigned)blocks);
   else if (cache->type == GPT2HIP_F16)
@@ -1905,7 +1916,12 @@ int attention_decode_paged_status(float* out, const GPT2PagedCache* cache, const
     launch_attend<bf16>(a, plan, (unsigned)blocks);
   G2_LAUNCH_CHECK("attention_decode_paged");
   if (weights && !a.weigh_here) {
-    hipLaunchKernelGGL(attention_paged_weights_kernel, dim3((unsigned)weighs), dim3(kWeighPositions), 0, stream(), a);
+    if (too_many(weighs, kWeighPositions))
+      hipLaunchKernelGGL(attention_paged_weights_kernel<true>, dim3(0xffffffffu / kWeighPositions), dim3(kWeighPositions), 0,
+                         stream(), a, (unsigned)weighs);
+    else
+      hipLaunchKernelGGL(attention_paged_weights_kernel<false>, dim3((unsigned)weighs), dim3(kWeighPositions), 0, stream(), a,
+                         (unsigned)weighs);
     G2_LAUNCH_CHECK("attention_decode_paged (weights)");
   }
   return GPT2HIP_OK;
@@ -1945,7 +1961,8 @@ int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, 
   const bool together = most <= 4096 && (4LL * budget <= 3LL * from.capacity || pairs * groups4 <= 1024);
   e.groups = together ? (int)groups4 : (budget + e.rows - 1) / e.rows;
   const long long copies = together ? pairs * e.groups : (pairs * e.groups + 3) / 4;
-  if (pairs > 0x7fffffffLL || copies > 0x7fffffffLL) return fail(GPT2HIP_EINVAL, "kv_evict_paged: grid too large");
+  if (too_many(copies, 256) || (!together && too_many(pairs, 16 * kWave)))
+    return fail(GPT2HIP_EINVAL, "kv_evict_paged: grid too large (B=%d, budget=%d)", B, budget);
 #define G2_UNITS(KERNEL)                                                                           \
   if (unit == 16 && e.row_bytes % 128 == 0) /* whole cache lines */                                \
     KERNEL(16, true);                                                                              \

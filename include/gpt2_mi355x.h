@@ -227,7 +227,8 @@ int matmul_forward_argmax_noalloc_status(int* ids, const float* inp, const float
  * output stay as they were.  Table entries outside [0, num_pages) are never followed: see each
  * call; nor are entries behind a sequence's last position, which may hold anything.  Nothing is
  * allocated, nothing synchronises, nothing is kept between calls: the calls can be captured in a
- * graph. */
+ * graph.  A call that would need 2^32 threads in one launch (64 per row stored, 256 or 512 per
+ * sequence and kv head attended to, ...) is refused. */
 enum { GPT2HIP_F32 = 0, GPT2HIP_F16 = 1, GPT2HIP_BF16 = 2 };
 typedef struct {
   void* keys;       /* (num_pages, kv_heads, page_size, head_size) of `type`, on the device */
