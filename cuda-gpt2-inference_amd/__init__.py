@@ -375,6 +375,9 @@ def attention_forward(out, qkvr, att, inp, B, T, C, NH):
                                           NH), "attention_forward")
 
 
+_INT_MAX = 2**31 - 1  # a C int takes any whole number and drops what is above its 32 bits
+
+
 class PagedCache:
     """A key/value cache in pages (GPT2PagedCache in the header).
 
@@ -392,6 +395,8 @@ class PagedCache:
                              f"{tuple(keys.shape)}, {tuple(values.shape)}")
         if table.dim() != 2:
             raise ValueError(f"table is (B, max_pages), got {tuple(table.shape)}")
+        if max(*keys.shape, *table.shape) > _INT_MAX:
+            raise ValueError(f"sizes have 32 bits, got {tuple(keys.shape)} and {tuple(table.shape)}")
         self.keys, self.values, self.table = keys, values, table
         pages, heads, size, channels = keys.shape
         self._c = GPT2PagedCache(_ptr(keys), _ptr(values), _i32(table), types[keys.dtype], pages, size,
@@ -426,7 +431,10 @@ def _rows(inp, cache, count, floats):
     if len(shape) != 2 or shape[0] < count or shape[1] < floats or (shape[1] > 1 and strides[1] != 1):
         raise ValueError(f"expected {count} rows of {floats} consecutive floats, got {tuple(shape)} with strides {strides}")
     # the stride of a single row says nothing
-    return inp.data_ptr(), strides[0] if count > 1 else max(strides[0], floats)
+    stride = strides[0] if count > 1 else max(strides[0], floats)
+    if stride > _INT_MAX or not 0 <= floats <= _INT_MAX or not 0 <= count <= _INT_MAX:
+        raise ValueError(f"counts and strides have 32 bits, got {count} rows of {floats} floats at a stride of {stride}")
+    return inp.data_ptr(), stride
 
 
 def _space(workspace, cache):
@@ -466,7 +474,7 @@ def attention_decode_paged_workspace(cache, B, NH, weights=False):
     zeroed on the launchers' stream (set_stream), whatever torch's current one is: calls on that
     stream find it zero, one on another stream has to be ordered behind it."""
     import torch
-    n = lib().attention_decode_paged_workspace(cache._ref, B, NH, int(weights))
+    n = lib().attention_decode_paged_workspace(cache._ref, B, NH, int(weights)) if 0 < B <= _INT_MAX and 0 < NH <= _INT_MAX else 0
     if n == 0:
         raise GPT2HipError(f"attention_decode_paged_workspace: bad arguments B={B} NH={NH} kv_heads={cache.kv_heads}")
     device = cache.keys.device
@@ -502,6 +510,8 @@ def kv_evict_paged(dst, src, kept, weights_out, lengths_out, weights_in, lengths
     others, each kv head for itself), copied from the pages of src into those of dst."""
     _on_its_gpu(src, B)
     _on_its_gpu(dst, B)
+    if not 0 <= recent <= _INT_MAX or budget > _INT_MAX:
+        raise GPT2HipError(f"kv_evict_paged: bad shape budget={budget} recent={recent}")
     f, i = src._float, src._int
     _check(lib().kv_evict_paged_status(dst._ref, src._ref, _array(kept, src, i, (B, src.kv_heads, budget), "kept"),
                                        _array(weights_out, src, f, (B, dst.kv_heads, dst.capacity), "weights_out"),

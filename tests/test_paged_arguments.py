@@ -92,3 +92,69 @@ def test_a_workspace_is_zeroed_on_the_stream_of_the_launchers(cache, library, mo
     space = g2.attention_decode_paged_workspace(cache, 2, 4)
     assert space.nbytes == g2.PAGED_COUNTER_BYTES + 1024 and not space.any()
     assert order == [launchers or 0]
+
+
+class Rows:
+    """A float32 array of any shape and strides on GPU 1, without its memory."""
+
+    dtype = torch.float32
+
+    def __init__(self, shape, strides):
+        self.shape, self.strides = shape, strides
+
+    def stride(self):
+        return self.strides
+
+    def get_device(self):
+        return 1
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+WRAP = 1 << 32  # what a C int cannot tell from 0
+
+
+def test_strides_and_counts_beyond_a_c_int_are_refused(cache, library):
+    starts, lengths = OnGpu.of((3,), torch.int32), OnGpu.of((2,), torch.int32)
+    step(cache, inp=Rows((2, 512), (2 ** 31 - 1, 1)))
+    g2.kv_store_paged(cache, Rows((5, 512), (512, 1)), starts, lengths, 5, 2, 4)
+    del library.calls[:]
+    for strides in ((WRAP + 512, 1), (2 ** 31, 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            step(cache, inp=Rows((2, 512), strides))
+        with pytest.raises(ValueError, match="32 bits"):
+            g2.kv_store_paged(cache, Rows((5, 512), strides), starts, lengths, 5, 2, 4)
+    for N in (WRAP + 5, 2 ** 31, -WRAP + 5):
+        with pytest.raises(ValueError, match="32 bits"):
+            g2.kv_store_paged(cache, Rows((WRAP + 9, 512), (512, 1)), starts, lengths, N, 2, 4)
+    for NH in (WRAP + 4, -WRAP + 4):
+        with pytest.raises(ValueError, match="32 bits"):
+            g2.kv_store_paged(cache, Rows((5, 64 * WRAP + 512), (512, 1)), starts, lengths, 5, 2, NH)
+    assert not library.calls
+
+
+def test_evict_and_workspace_refuse_numbers_beyond_a_c_int(cache, library):
+    other = g2.PagedCache(cache.keys, cache.values, OnGpu.of((2, 4), torch.int32))
+    arrays = [OnGpu.of((2, 2, 16), torch.int32), OnGpu.of((2, 2, 64)), OnGpu.of((2,), torch.int32), OnGpu.of((2, 2, 64)),
+              OnGpu.of((2,), torch.int32)]
+    g2.kv_evict_paged(other, cache, *arrays, 2, 16, 4)
+    del library.calls[:]
+    for recent in (WRAP + 4, -WRAP + 4):
+        with pytest.raises(g2.GPT2HipError, match="recent"):
+            g2.kv_evict_paged(other, cache, *arrays, 2, 16, recent)
+    with pytest.raises(g2.GPT2HipError, match="budget"):
+        g2.kv_evict_paged(other, cache, Rows((2, 2, WRAP + 16), (2 * WRAP, WRAP, 1)), *arrays[1:], 2, WRAP + 16, 4)
+    for B, NH in ((WRAP + 2, 4), (2, WRAP + 4), (-WRAP + 2, 4)):
+        with pytest.raises(g2.GPT2HipError, match="arguments"):
+            g2.attention_decode_paged_workspace(cache, B, NH)
+    assert not library.calls
+
+
+def test_a_cache_of_more_pages_than_a_c_int_counts_is_refused(cache):
+    class Wide(OnGpu):
+        shape = property(lambda self: torch.Size((WRAP + 8, 2, 16, 64)))
+
+    keys = torch.zeros((8, 2, 16, 64)).as_subclass(Wide)
+    with pytest.raises(ValueError, match="32 bits"):
+        g2.PagedCache(keys, keys, OnGpu.of((2, 4), torch.int32))
