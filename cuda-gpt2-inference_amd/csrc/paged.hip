@@ -142,7 +142,7 @@ __global__ __launch_bounds__(256) void kv_store_paged_kernel(Pages pg, const flo
   }
   // in front of the first row or behind the last; starts that do not ascend are nobody's either
   if (b < 0 || b >= B || begin > r || starts[b + 1] <= r) return;
-  const long long pos = (long long)n + (r - begin);
+  const long long pos = (long long)n + r - begin;  // begin may be below 0
   if (n < 0 || pos >= pg.capacity) return;
   bool ok = true;
   const unsigned row0 = pg.row(b, 0, (int)pos, ok);

@@ -36,3 +36,27 @@ def test_attend_weights_of_a_table_wider_than_a_launch():
     assert ((out[0].cpu().double() - exp).abs() <= tol).all()
     assert ((wide[0, :, : n + 1].cpu().double() - p).abs() <= ptol).all()
     assert not wide[:, :, n + 1: n + 1000].any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_store_with_starts_far_in_front_of_the_rows(kind):
+    """A sequence whose first row lies 2^31 in front of row 0: its positions do not fit and nothing
+    is stored; one that begins a little in front of row 0 has its later rows here."""
+    dtype = {"f32": torch.float32, "bf16": torch.bfloat16}[kind]
+    g = torch.Generator().manual_seed(81)
+    rows = torch.randn((5, 2 * 2 * 8), generator=g)
+    for start, length in ((-(1 << 31), 0), (-(1 << 31), (1 << 31) - 1), (-(1 << 31) + 3, 5), (-2, 7), (-2, 0), (0, (1 << 31) - 1)):
+        say(f"starts {start} lengths {length}")
+        keys = torch.full((4, 2, 4, 8), 9.0, dtype=dtype, device="cuda")
+        values = keys.clone()
+        table = torch.tensor([[2, 0, 3], [1, 1, 1]], dtype=torch.int32).cuda()
+        g2.kv_store_paged(g2.PagedCache(keys, values, table), rows.cuda(), torch.tensor([start, 3, 3], dtype=torch.int32).cuda(),
+                          torch.tensor([length, 0], dtype=torch.int32).cuda(), 5, 2, 0)
+        want_k, want_v = torch.full((4, 2, 4, 8), 9.0, dtype=dtype), torch.full((4, 2, 4, 8), 9.0, dtype=dtype)
+        for r in range(3):
+            pos = length + r - start
+            if pos < 12:
+                at, slot = int(table[0, pos // 4]), pos % 4
+                want_k[at, :, slot] = rows[r, :16].view(2, 8).to(dtype)
+                want_v[at, :, slot] = rows[r, 16:].view(2, 8).to(dtype)
+        assert torch.equal(keys.cpu(), want_k) and torch.equal(values.cpu(), want_v)
