@@ -261,6 +261,8 @@ int kv_store_paged_status(const GPT2PagedCache* cache, const float* inp, int inp
  * attention_forward.  An infinity among the values gives that infinity in its channel (infinities
  * of both signs, or a NaN, a NaN) for every query head that weighs it with 2^-126 or more; where
  * the weight is below, an infinity or a NaN; where it is 0 exactly, from a score of -inf, a NaN.
+ * Weighted values are summed before the division: where such a sum passes fp32 (values near 1e38,
+ * that is), the output is not finite.
  * weights_in, weights_out (both or neither; may be the same array): (B, kv_heads, max_pages *
  * page_size) accumulated attention weights, for kv_evict_paged.  weights_out[b][h][i] becomes
  * weights_in[b][h][i] (0 for the position just appended) plus the weight that position i got

@@ -150,3 +150,31 @@ def test_outputs_beside_infinities_keep_their_bits(kind):
     assert (outs[1][:, 0, :, 11] == INF).all()
     outs[1][:, 0, :, 11] = outs[0][:, 0, :, 11]
     assert same_bits(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("NH", [1, 8])
+def test_sums_of_values_that_pass_fp32_are_not_finite(kind, NH):
+    """Values are summed before the division: finite ones whose sum passes 2^128 leave an infinity or a
+    NaN in their channel, never another number, and no trace in the other channels."""
+    say(f"overflow {kind} NH={NH}")
+    n = 2000
+    c = Case(9, kind, 1, NH, 1, 64, 16, [n], n + 1)
+    c.inp[:, : NH * 64] = 0
+    plain = c.v64[0][0].clone()
+    for i in range(n):
+        put(c, 0, i, 0, 5, 3e38 if i % 64 < 32 else -1.5e38)   # both signs in every wave
+        put(c, 0, i, 0, 6, 3e38)
+        put(c, 0, i, 0, 7, 3e38 if i < n // 2 else -1.5e38)
+    cache = c.gpu()
+    for ws in (None, g2.attention_decode_paged_workspace(cache, 1, NH)):
+        out = torch.zeros((1, NH * 64), device="cuda")
+        g2.attention_decode_paged(out, cache, c.inp[:, : NH * 64].contiguous().cuda(), c.dl, 1, NH, append=False, workspace=ws)
+        got = out.cpu().double().view(NH, 64)
+        assert not torch.isfinite(got[:, 6]).any()
+        for d in (5, 7):
+            # not finite, or right where a sum happens to stay below 2^128
+            exact = float(c.v64[0][0, :, d].mean())
+            assert (~torch.isfinite(got[:, d]) | ((got[:, d] - exact).abs() <= 2.0 ** -24 * 4 * n * 3e38)).all()
+        others = [d for d in range(64) if d not in (5, 6, 7)]
+        assert ((got[:, others] - plain[:, others].mean(0)).abs() <= 4 * n * 2.0 ** -24 * plain[:, others].abs().mean(0)).all()
