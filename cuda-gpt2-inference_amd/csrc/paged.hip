@@ -101,8 +101,9 @@ struct Pages {
 // One wave per row of the prompts: it finds the row's sequence by counting the starts that are
 // not behind it, 64 at a time, and moves the row's keys and values, VEC floats per lane and step.
 // A copy, bound by memory: 8 prompts of 129-1023 rows, 12 heads, fp32: 13.5 us = 4.8 TB/s; 4 of
-// 4001-8192 rows, 8 heads of 128, bf16: 57.8 us = 5.4 TB/s (a 2 GiB copy reaches 4.9).  16-bit rows
-// are stored past the caches (12 x 5-496 rows, 20 heads, fp16: 13.8 -> 11.9 us; fp32 gains nothing).
+// 4001-8192 rows, 8 heads of 128, bf16: 57.5 us = 5.5 TB/s (a streaming copy of 192 MiB reaches 6.2,
+// one that writes half of what it reads 6.3-6.5, torch's copy of 2 GiB 4.9).  16-bit rows are stored
+// past the caches (12 x 5-496 rows, 20 heads, fp16: 13.8 -> 11.9 us; fp32 gains nothing).
 // The first loads of the row are under way while its place is looked up.
 template <class E, int VEC>
 __global__ __launch_bounds__(256) void kv_store_paged_kernel(Pages pg, const float* __restrict__ inp, int stride,
@@ -1714,7 +1715,11 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH, bool weigh
   const long long each = capacity * row_bytes;  // of keys and values, per group
   // As many workgroups as compute units, or, where that is less than two per sequence, there is
   // much to do and whole sequences would not fill the units evenly, twice as many.  A range is
-  // worth a workgroup from 64 KB on.
+  // worth a workgroup from 64 KB on.  The capacity is all that is known of the lengths here: dealing
+  // to twice as many gains where they are uneven (8 of 32 heads of 128, bf16, 24 sequences of
+  // 100-6000: 94.7 -> 68.9 us) and costs where they are even (24 of 1535: 31.9 -> 44.6; 36 of 4071:
+  // 138.0 -> 139.5); from 205 to 256 groups the loss is taken to matter more (28 of 1535: 33.5
+  // whole, 45.6 dealt; but 28 of 1-8900: 141 whole, 106 dealt).
   p.min_range = (int)((65536 / row_bytes + 63) & ~63LL);
   if (p.min_range < 128) p.min_range = 128;
   const long long per = (long long)c->kv_heads * p.chunks, ranges = capacity / p.min_range;  // ranges of a sequence, at most
@@ -1724,10 +1729,10 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH, bool weigh
   } else {
     // Splitting costs 4 us (parts to memory, the counter, parts back) and, with weights, a second
     // launch.  A workgroup takes 18 ns for a KB of cache, 27 in the matrix kernel, and all of them
-    // together at least 0.12 ns per KB.  (12 heads, fp32: whole or split, one sequence of 384
-    // positions 6.7 or 8.3 us, of 640 9.2 or 8.4; 8 of 896 13.3 or 15.2, of 1800 23.1 or 21.7,
-    // with weights 25.9 or 25.0.  4 sequences, 8 of 32 heads of 128, bf16: 384 11.3 or 11.9, with
-    // weights 12.4 or 15.3; 640 14.9 or 11.9, with weights 16.0 or 15.3.)
+    // together at least 0.12 ns per KB.  (12 heads, fp32: whole or split, one sequence of 383
+    // positions 6.4 or 8.0 us, of 895 10.9 or 8.5; 8 of 895 13.3 or 15.2, of 1791 23.2 or 20.5, with
+    // weights 25.1 or 24.3.  4 sequences, 8 of 32 heads of 128, bf16: 383 10.1 or 11.1, with weights
+    // 11.5 or 14.8; 639 14.5 or 11.7, with weights 15.8 or 15.2.)
     const double alone = p.matrix ? 27. : 18., parts = (double)(slots < B * ranges ? slots : B * ranges) / B;
     const double split = parts > 1. ? alone / parts : alone, together = 0.12 * (double)groups;
     if ((double)each / 1024. * (alone - (split > together ? split : together)) < (weights ? 5300. : 4000.)) slots = 0;
@@ -1735,12 +1740,12 @@ static AttendPlan plan_attend(const GPT2PagedCache* c, int B, int NH, bool weigh
   if (slots > B * ranges) slots = B * ranges;
   if (B > kMostSplit || groups * kCounterStride * 4 > GPT2HIP_PAGED_COUNTER_BYTES) slots = 0;
   p.slots = slots > B ? (int)slots : B;
-  // Four waves instead of eight for many short caches (64 sequences of 12 heads, bf16, up to 100
-  // positions: 7.0 against 9.3 us; 64 of 16 heads of 128 channels, up to 2000: 135 against 130)
+  // Four waves instead of eight for many short caches (64 sequences of 12 heads, bf16, of 100
+  // positions: 7.2 against 9.9 us; 64 of 16 heads of 128, of 2000, the other way: 164 against 161)
   // and where eight would take all of a unit's registers: the matrix kernel from 257 groups on
-  // (8 of 32 heads, fp32, 55 sequences: 20.3 against 25.2 us) and for head sizes above 128 -- or
-  // where four have one tile each and no more (30 sequences of 8 of 32 heads, fp16, up to 60: 6.9
-  // against 7.4 us).
+  // (8 of 32 heads, fp32, 55 sequences of 350: 18.0 against 22.9 us) and for head sizes above 128
+  // -- or where four have one tile each and no more (30 sequences of 8 of 32 heads of 128, fp16, of
+  // 60: 7.3 against 7.5 us).
   p.waves = 8;
   if (!p.rows16 || (groups > 512 && each < 768 * 1024)) p.waves = 4;
   if (p.matrix && (groups > 256 || (capacity <= 128 && type_bytes(c->type) == 2) || c->head_size > 128)) p.waves = 4;
@@ -1955,9 +1960,11 @@ int kv_evict_paged_status(const GPT2PagedCache* dst, const GPT2PagedCache* src, 
   const int unit = rows_by_16(src) && rows_by_16(dst) ? 16 : (int)type_bytes(src->type);
   e.rows = copy_rows(e.row_bytes, unit);
   const int most = from.capacity - recent;  // weights that can take part
-  // Choice and copy in one launch, the choice made again by every workgroup: up to 4096 weights,
-  // and not where many workgroups would copy nearly everything (48 pairs, 2000 -> 1000 positions:
-  // 17.2 -> 14.0 us; 768 pairs, 185 -> 168; but 768 pairs, 4000 -> 3600: 318 -> 375).
+  // Choice and copy in one launch, the choice made again by every workgroup: up to 4096 weights
+  // (48 pairs, bf16, 2000 -> 1000 positions: 15.4 -> 13.0 us; 768 pairs, 4000 -> 2000: 178 -> 168).
+  // Where many workgroups would copy nearly everything it is two launches, a bound from before the
+  // first bits were counted in LDS: now one launch is the faster there too (768 pairs, 4000 -> 3600:
+  // 301 against 313 us; fp32, 250 -> 225: 43 against 68).
   const long long pairs = (long long)B * KVH, groups4 = (budget + 4 * e.rows - 1) / (4 * e.rows);
   const bool together = most <= 4096 && (4LL * budget <= 3LL * from.capacity || pairs * groups4 <= 1024);
   e.groups = together ? (int)groups4 : (budget + e.rows - 1) / e.rows;
