@@ -36,6 +36,8 @@ def test_attend_weights_of_a_table_wider_than_a_launch():
     assert ((out[0].cpu().double() - exp).abs() <= tol).all()
     assert ((wide[0, :, : n + 1].cpu().double() - p).abs() <= ptol).all()
     assert not wide[:, :, n + 1: n + 1000].any()
+    del wide, ws, cache
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
